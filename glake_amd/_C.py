@@ -13,7 +13,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # VTKV_LIBRARY_PATH selects another build of the same library (e.g. a tuning variant)
 LIB_PATH = os.environ.get("VTKV_LIBRARY_PATH") or os.path.join(_HERE, "lib", "libvtkv.so")
 
-F32, BF16, F16, FP8_E4M3 = 0, 1, 2, 3
+F32, BF16, F16, FP8_E4M3, INT4 = 0, 1, 2, 3, 4
 D2H, H2D, D2D = 0, 1, 2
 OK, EINVAL, EHIP, ENOMEM, ESTATE = 0, -1, -2, -3, -4
 
@@ -76,6 +76,8 @@ SIGNATURES = {
     "vtkv_memcpy_d2h": (_i, [_p, _u64, _i64]),
     "vtkv_memcpy_h2d_async": (_i, [_u64, _p, _i64, _p]),
     "vtkv_reshape_and_cache": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i64, _i64, _i, _i, _f, _f, _p]),
+    "vtkv_kv_row_bytes": (_i64, [_i, _i, _i]),
+    "vtkv_read_cached_rows": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i64, _i64, _i, _i, _p]),
     "vtkv_reshape_and_cache_paged": (_i, [_p, _p, _p, _p, _p, _i, _i, _i, _i, _i64, _i64, _i, _p]),
     "vtkv_swap_blocks": (_i, [_p, _p, _i64, _p, _i, _i, _p]),
     "vtkv_swap_ranges": (_i, [_p, _p, _p, _i, _i, _i64, _i, _p]),
@@ -98,6 +100,11 @@ SIGNATURES = {
     "vtkv_prefill_unit_tokens": (_i, [_i, _i, _i]),
     "vtkv_prefill_unit_tokens_for": (_i, [_i, _i, _i, _i]),
     "vtkv_prefill_attention": (_i, [_p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i64, _f, _i, _p, _i, _i, _i, _f, _f, _p]),
+    "vtkv_accumulate_attention_weights_workspace_bytes": (_i64, [_i, _i, _i]),
+    "vtkv_accumulate_attention_weights": (_i, [_p, _i64, _i64, _i64, _p, _p, _p, _p, _i, _i, _i, _i, _i64, _f, _i, _p, _i,
+                                               _i, _f, _p, _i64, _p]),
+    "vtkv_evict_rows_workspace_bytes": (_i64, [_i, _i, _i, _i, _i]),
+    "vtkv_evict_rows": (_i, [_p, _p, _p, _i64, _i64, _i64, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p, _i64, _p]),
     "vtkv_set_fused_merge": (_i, [_i]),
     "vtkv_set_head_major": (_i, [_i]),
     "vtkv_set_kernel_timing": (_i, [_i]),

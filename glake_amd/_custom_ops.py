@@ -47,13 +47,45 @@ def _kv_dtype(kv_cache_dtype: str, model_dtype: int) -> int:
         return model_dtype
     if kv_cache_dtype in ("fp8", "fp8_e4m3"):
         return _C.FP8_E4M3
+    if kv_cache_dtype == "int4":
+        return _C.INT4
     raise _C.VtkvError(_C.EINVAL, f"Unsupported data type of kv cache: {kv_cache_dtype}")
+
+
+def _int4_scales(kv_cache_dtype: str, *scales) -> None:
+    """A 4-bit cache carries its scales in its rows: a per-tensor scale beside them is a mistake of the caller."""
+    if kv_cache_dtype == "int4" and any(s is not None and s != 1.0 for s in scales):
+        raise _C.VtkvError(_C.EINVAL, "an int4 cache holds its own scales: kv_scale, k_scale and v_scale must be 1")
 
 
 def _require_cuda(*tensors) -> None:
     for t in tensors:
         if isinstance(t, torch.Tensor) and not t.is_cuda:
             raise _C.VtkvError(_C.EINVAL, "tensor must live on the GPU")
+
+
+def _per_sequence(num_seqs: int, seq_lens: torch.Tensor, slot_mapping: torch.Tensor) -> None:
+    """One int32 length and one int64 slot per sequence, on the current device (whose stream the call runs on)."""
+    _require_cuda(seq_lens, slot_mapping)
+    if seq_lens.dtype != torch.int32 or slot_mapping.dtype != torch.int64:
+        raise _C.VtkvError(_C.EINVAL, "seq_lens must be int32 and slot_mapping int64")
+    for t in (seq_lens, slot_mapping):
+        if t.dim() != 1 or t.shape[0] != num_seqs or not t.is_contiguous():
+            raise _C.VtkvError(_C.EINVAL, "seq_lens and slot_mapping hold one entry per sequence, contiguous")
+
+
+def _on_current_device(*tensors) -> None:
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and t.is_cuda and t.device.index != torch.cuda.current_device():
+            raise _C.VtkvError(_C.EINVAL, f"tensor on {t.device}, but the current device is {torch.cuda.current_device()}")
+
+
+def _slopes(alibi_slopes: Optional[torch.Tensor], num_heads: int, device: torch.device) -> Optional[torch.Tensor]:
+    if alibi_slopes is None:
+        return None
+    if alibi_slopes.numel() != num_heads:
+        raise _C.VtkvError(_C.EINVAL, "alibi_slopes must hold one slope per query head")
+    return alibi_slopes.to(device=device, dtype=torch.float32).contiguous()
 
 
 # Scratch for the attention's partial results, grown on demand: one per device and stream, because calls
@@ -77,6 +109,19 @@ def _workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     return ws
 
 
+def _int4_query(out: torch.Tensor, query: torch.Tensor) -> None:
+    if out.shape != query.shape:
+        raise _C.VtkvError(_C.EINVAL, "out must be shaped like query")
+    if query.stride(2) != 1 or query.stride(1) != query.shape[2]:
+        raise _C.VtkvError(_C.EINVAL, "query rows must be contiguous in (head, dim)")
+
+
+def _scratch(nbytes: int, device: torch.device) -> torch.Tensor:
+    """Scratch of one call, contents undefined: from torch's allocator, which hands it on in stream order and gives a
+    graph under capture memory of its own, so that neither streams nor graphs share it."""
+    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=device)
+
+
 # --------------------------------------------------------------------------------------- attention
 def paged_attention_v1(
     out: torch.Tensor,
@@ -98,20 +143,28 @@ def paged_attention_v1(
     """Fork signature (csrc/ops.h:6-19): key_cache / value_cache are the device address of
     (or an int64 tensor holding) the per-slot base pointers, ``slot_mapping`` holds each
     sequence's slot; ``block_size`` must be 1 (vllm/attention/ops/paged_attn.py:105).
-    ``kv_scale`` scales K (and V unless ``v_scale`` is given) for an fp8 cache.  ``out`` has the
-    query's dtype, or float32 to receive the result before its final rounding."""
+    ``kv_scale`` scales K (and V unless ``v_scale`` is given) for an fp8 cache.  ``kv_cache_dtype="int4"`` reads
+    4-bit rows (``reshape_and_cache`` writes them; their scales are in the rows, so ``kv_scale`` stays 1); there a
+    sequence of length 0 gets zeros.  ``out`` has the query's dtype, or float32 to receive the result before its
+    final rounding."""
     if block_size != 1:
         raise _C.VtkvError(_C.EINVAL, f"Unsupported block size: {block_size} (contiguous ranges use 1)")
     _require_cuda(out, query, seq_lens, slot_mapping)
     num_seqs, num_heads, head_size = query.shape
     if not out.is_contiguous():
         raise _C.VtkvError(_C.EINVAL, "out must be contiguous")
+    if kv_cache_dtype == "int4":
+        _int4_scales(kv_cache_dtype, kv_scale, v_scale)
+        _per_sequence(num_seqs, seq_lens, slot_mapping)
+        _on_current_device(out, query, key_cache, value_cache, seq_lens, slot_mapping)
+        _int4_query(out, query)
+        alibi_slopes = _slopes(alibi_slopes, num_heads, query.device)
     if seq_lens.dtype != torch.int32 or slot_mapping.dtype != torch.int64:
         raise _C.VtkvError(_C.EINVAL, "seq_lens must be int32 and slot_mapping int64")
     qd = _dt(query)
     lib = _C.lib()
     need = lib.vtkv_decode_attention_workspace_bytes(num_seqs, num_heads, head_size, max_seq_len, partition_tokens)
-    ws = _workspace(need, query.device)
+    ws = _scratch(need, query.device) if kv_cache_dtype == "int4" else _workspace(need, query.device)
     if alibi_slopes is not None:
         alibi_slopes = alibi_slopes.to(device=query.device, dtype=torch.float32)
     _C.check(lib.vtkv_decode_attention(
@@ -239,6 +292,13 @@ def prefill_attention(
     ``query`` / ``out`` are [num_query_tokens, num_heads, head_size], sequences packed in order;
     ``query_lens`` / ``seq_lens`` are host lists; ``slot_mapping`` holds each sequence's slot."""
     _require_cuda(out, query, slot_mapping)
+    if kv_cache_dtype == "int4":
+        _int4_scales(kv_cache_dtype, kv_scale, v_scale)
+        _on_current_device(out, query, key_cache, value_cache, slot_mapping)
+        _int4_query(out, query)
+        alibi_slopes = _slopes(alibi_slopes, query.shape[1], query.device)
+        if slot_mapping.shape[0] < len(seq_lens) or not slot_mapping.is_contiguous():
+            raise _C.VtkvError(_C.EINVAL, "slot_mapping must hold one slot per sequence, contiguous")
     num_tokens, num_heads, head_size = query.shape
     if not out.is_contiguous() or out.shape != query.shape:
         raise _C.VtkvError(_C.EINVAL, "out must be contiguous and shaped like query")
@@ -342,8 +402,17 @@ def reshape_and_cache(
 ) -> None:
     """vTensor scatter (vllm/_custom_ops.py:238-252): ``key_cache`` / ``value_cache`` are
     int64 device tensors of per-slot base addresses, ``slot_m`` the byte offset of each
-    sequence's next row, ``slot_mapping`` its slot."""
+    sequence's next row, ``slot_mapping`` its slot.  ``kv_cache_dtype="int4"`` quantises bf16 and fp16 rows to 4
+    bits with a scale and a zero per token and kv head; such a row takes ``worker.step.kv_row_bytes(num_kv_heads,
+    head_size, "int4")`` bytes."""
     _require_cuda(key, value, slot_m, slot_mapping)
+    if kv_cache_dtype == "int4":
+        _int4_scales(kv_cache_dtype, k_scale, v_scale)
+        _on_current_device(key, value, key_cache, value_cache, slot_m, slot_mapping)
+        if key.dtype != value.dtype or not (slot_m.is_contiguous() and slot_mapping.is_contiguous()):
+            raise _C.VtkvError(_C.EINVAL, "key and value must have one dtype, slot_m and slot_mapping be contiguous")
+        if slot_m.shape != slot_mapping.shape:
+            raise _C.VtkvError(_C.EINVAL, "slot_m and slot_mapping must hold one entry per sequence")
     if slot_m.dtype != torch.int64 or slot_mapping.dtype != torch.int64:
         raise _C.VtkvError(_C.EINVAL, "slot_m and slot_mapping must be int64")
     for t in (seq_lens, cache_seq_lens):
@@ -359,6 +428,129 @@ def reshape_and_cache(
         _ptr(seq_lens), _ptr(cache_seq_lens), slot_mapping.shape[0], int(max_seq_len), num_kv_heads, head_size,
         key.stride(0), value.stride(0), sd, _kv_dtype(kv_cache_dtype, sd), float(k_scale), float(v_scale),
         _stream()))
+
+
+def read_cached_rows(
+    key: torch.Tensor,
+    value: torch.Tensor,
+    key_cache: Union[int, torch.Tensor],
+    value_cache: Union[int, torch.Tensor],
+    slot_m: torch.Tensor,
+    slot_mapping: torch.Tensor,
+    seq_lens: Optional[torch.Tensor],
+    cache_seq_lens: Optional[torch.Tensor],
+    max_seq_len: int,
+    num_kv_heads: int,
+    head_size: int,
+    kv_cache_dtype: str = "int4",
+) -> None:
+    """The inverse of ``reshape_and_cache`` for a 4-bit cache, with its arguments: ``key`` / ``value`` receive the
+    cached rows as values (code * scale + zero, rounded to their dtype: float32, bfloat16 or float16).  ``slot_m`` is
+    the byte offset of the first row to read of each sequence (negative: none).  No counterpart in the reference."""
+    if kv_cache_dtype != "int4":
+        raise _C.VtkvError(_C.EINVAL, f"read_cached_rows reads int4 caches, not {kv_cache_dtype}")
+    _require_cuda(key, value, slot_m, slot_mapping, seq_lens, cache_seq_lens)
+    _on_current_device(key, value, key_cache, value_cache, slot_m, slot_mapping, seq_lens, cache_seq_lens)
+    if slot_m.dtype != torch.int64 or slot_mapping.dtype != torch.int64 or slot_m.shape != slot_mapping.shape:
+        raise _C.VtkvError(_C.EINVAL, "slot_m and slot_mapping must be int64, one entry per sequence")
+    for t in (seq_lens, cache_seq_lens):
+        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous()):
+            raise _C.VtkvError(_C.EINVAL, "seq_lens and cache_seq_lens must be int32 and contiguous")
+    if key.dtype != value.dtype or not (slot_m.is_contiguous() and slot_mapping.is_contiguous()):
+        raise _C.VtkvError(_C.EINVAL, "key and value must have one dtype, slot_m and slot_mapping be contiguous")
+    key = key.view(-1, num_kv_heads, head_size)
+    value = value.view(-1, num_kv_heads, head_size)
+    if key.stride(2) != 1 or key.stride(1) != head_size or value.stride(2) != 1 or value.stride(1) != head_size:
+        raise _C.VtkvError(_C.EINVAL, "key/value rows must be contiguous in (head, dim)")
+    _C.check(_C.lib().vtkv_read_cached_rows(
+        _ptr(key), _ptr(value), _ptr(key_cache), _ptr(value_cache), _ptr(slot_m), _ptr(slot_mapping), _ptr(seq_lens),
+        _ptr(cache_seq_lens), slot_mapping.shape[0], int(max_seq_len), num_kv_heads, head_size, key.stride(0),
+        value.stride(0), _dt(key), _C.INT4, _stream()))
+
+
+# --------------------------------------------------------------------------------------- a bounded cache
+def _weights_of(weights: torch.Tensor, num_kv_heads: int, max_seq_len: int) -> None:
+    if weights.dtype != torch.float32 or weights.dim() != 3 or weights.shape[1] != num_kv_heads \
+            or weights.shape[2] < max_seq_len or (weights.shape[2] > 1 and weights.stride(2) != 1):
+        raise _C.VtkvError(_C.EINVAL, "weights must be float32 [slots, num_kv_heads, >= max_seq_len] with contiguous rows")
+
+
+def accumulate_attention_weights(
+    weights: torch.Tensor,
+    query: torch.Tensor,
+    key_cache: Union[int, torch.Tensor],
+    num_kv_heads: int,
+    scale: float,
+    seq_lens: torch.Tensor,
+    max_seq_len: int,
+    slot_mapping: torch.Tensor,
+    alibi_slopes: Optional[torch.Tensor] = None,
+    kv_cache_dtype: str = "auto",
+    kv_scale: float = 1.0,
+) -> None:
+    """Adds to ``weights[slot, kv head, row]`` (float32, kept by the caller from step to step) what one query token per
+    sequence pays to each of its sequence's cached rows: the softmax weights that ``paged_attention_v1`` with the same
+    arguments multiplies V with, summed over the kv head's query heads.  The slots of a call are distinct.  ``evict_rows``
+    goes by these sums.  No counterpart in the reference."""
+    _require_cuda(weights, query)
+    num_seqs, num_heads, head_size = query.shape
+    _per_sequence(num_seqs, seq_lens, slot_mapping)
+    _weights_of(weights, num_kv_heads, max_seq_len)
+    _on_current_device(weights, query, key_cache, seq_lens, slot_mapping)
+    if query.stride(2) != 1 or query.stride(1) != head_size:
+        raise _C.VtkvError(_C.EINVAL, "query rows must be contiguous in (head, dim)")
+    _int4_scales(kv_cache_dtype, kv_scale)
+    qd = _dt(query)
+    lib = _C.lib()
+    alibi_slopes = _slopes(alibi_slopes, num_heads, query.device)
+    ws = _scratch(lib.vtkv_accumulate_attention_weights_workspace_bytes(num_seqs, num_heads, max_seq_len), query.device)
+    _C.check(lib.vtkv_accumulate_attention_weights(
+        _ptr(weights), weights.stride(0), weights.stride(1), weights.shape[0], _ptr(query), _ptr(key_cache),
+        _ptr(slot_mapping), _ptr(seq_lens), num_seqs, num_heads, num_kv_heads, head_size, query.stride(0), float(scale),
+        int(max_seq_len), _ptr(alibi_slopes), qd, _kv_dtype(kv_cache_dtype, qd), float(kv_scale), _ptr(ws),
+        ws.numel(), _stream()))
+
+
+def evict_rows(
+    key_cache: Union[int, torch.Tensor],
+    value_cache: Union[int, torch.Tensor],
+    weights: torch.Tensor,
+    seq_lens: torch.Tensor,
+    new_seq_lens: torch.Tensor,
+    keep_rows: int,
+    recent_rows: int,
+    max_seq_len: int,
+    slot_mapping: torch.Tensor,
+    num_kv_heads: int,
+    head_size: int,
+    kv_cache_dtype: str = "auto",
+    model_dtype: torch.dtype = torch.bfloat16,
+) -> None:
+    """Cuts every sequence of the batch that holds more than ``keep_rows`` rows back to ``keep_rows``, in place and each
+    kv head by itself: the last ``recent_rows`` rows stay, and of those before them the ones with the largest
+    ``weights[slot, kv head, row]`` (of equal ones the first).  With ``heavy = keep_rows - recent_rows``, rows below
+    ``heavy`` that stay keep their places, the others that stay fill the places of evicted ones in order, and the recent
+    rows move to ``[heavy, keep_rows)``.  ``weights`` moves with the rows and is zero behind them; ``new_seq_lens``
+    (which may be ``seq_lens``) receives the lengths.  The caller takes the rows off its own bookkeeping
+    (``KVcacheSegment.set_used_size``).  The rows of a head are not in the order of their tokens afterwards, which
+    attention without ALiBi does not notice; ranges that share chunks with another sequence must not be evicted from.
+    ``model_dtype`` is the type of the rows of an "auto" cache.  No counterpart in the reference."""
+    _require_cuda(weights, new_seq_lens)
+    num_seqs = slot_mapping.shape[0]
+    _per_sequence(num_seqs, seq_lens, slot_mapping)
+    _per_sequence(num_seqs, new_seq_lens, slot_mapping)
+    _weights_of(weights, num_kv_heads, max_seq_len)
+    _on_current_device(weights, key_cache, value_cache, seq_lens, new_seq_lens, slot_mapping)
+    if model_dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise _C.VtkvError(_C.EINVAL, f"unsupported model dtype {model_dtype}")
+    lib = _C.lib()
+    ws = _scratch(lib.vtkv_evict_rows_workspace_bytes(num_seqs, num_kv_heads, max_seq_len, keep_rows, recent_rows),
+                  weights.device)
+    _C.check(lib.vtkv_evict_rows(
+        _ptr(key_cache), _ptr(value_cache), _ptr(weights), weights.stride(0), weights.stride(1), weights.shape[0],
+        _ptr(slot_mapping), _ptr(seq_lens), _ptr(new_seq_lens), num_seqs, num_kv_heads, head_size,
+        _kv_dtype(kv_cache_dtype, _DTYPES[model_dtype]), int(keep_rows), int(recent_rows), int(max_seq_len), _ptr(ws),
+        ws.numel(), _stream()))
 
 
 def reshape_and_cache_paged(

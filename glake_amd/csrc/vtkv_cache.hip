@@ -10,6 +10,7 @@
 
 #include "vtkv_common.h"
 #include "vtkv_fp8.h"
+#include "vtkv_int4.h"
 
 namespace {
 
@@ -233,6 +234,9 @@ int vtkv_reshape_and_cache(const void *key, const void *value, const int64_t *k_
                            const int32_t *cache_seq_lens, int batch, int max_seq_len, int num_heads, int head_size,
                            int64_t key_stride, int64_t value_stride, int src_dtype, int kv_dtype, float k_scale,
                            float v_scale, void *stream) {
+  if (kv_dtype == VTKV_INT4)
+    return vtkv::int4_write_rows(key, value, k_ptrs, v_ptrs, slot_m, slot_ids, seq_lens, cache_seq_lens, batch, max_seq_len,
+                                 num_heads, head_size, key_stride, value_stride, src_dtype, stream);
   VTKV_REQUIRE(key && value && k_ptrs && v_ptrs && slot_m && slot_ids, "null argument");
   VTKV_REQUIRE(batch >= 0 && max_seq_len >= 1 && num_heads > 0 && head_size > 0, "bad sizes");
   VTKV_REQUIRE(max_seq_len == 1 || (seq_lens && cache_seq_lens), "seq_lens and cache_seq_lens are needed when max_seq_len > 1");
@@ -273,7 +277,7 @@ int vtkv_reshape_and_cache(const void *key, const void *value, const int64_t *k_
     else LAUNCH_FP8(VTKV_F16);
 #undef LAUNCH_FP8
   } else {
-    return vtkv::fail(VTKV_EINVAL, "kv_dtype %d must equal src_dtype %d or be FP8_E4M3", kv_dtype, src_dtype);
+    return vtkv::fail(VTKV_EINVAL, "kv_dtype %d must equal src_dtype %d or be FP8_E4M3 or INT4", kv_dtype, src_dtype);
   }
   VTKV_HIP(hipGetLastError());
   return VTKV_OK;

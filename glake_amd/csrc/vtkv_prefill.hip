@@ -31,6 +31,7 @@
 // an external flash-attention kernel (vllm/attention/backends/xformers.py:331-386).
 #include "vtkv_attn_common.h"
 #include "vtkv_common.h"
+#include "vtkv_int4.h"
 
 #include <type_traits>
 
@@ -548,6 +549,13 @@ int vtkv_prefill_attention(void *out, const void *q, const int64_t *k_ptrs, cons
                "num_heads %d must be a positive multiple of num_kv_heads %d", num_heads, num_kv_heads);
   const int d_index = size_index(head_size);
   VTKV_REQUIRE(d_index >= 0, "head_size %d is not supported (64, 80, 96, 112, 128, 256)", head_size);
+  if (kv_dtype == VTKV_INT4) {
+    const int per_unit = vtkv_prefill_unit_tokens_for(num_heads, num_kv_heads, head_size, kv_dtype);
+    VTKV_REQUIRE(per_unit > 0, "unsupported head counts");
+    return vtkv::int4_attention(out, q, k_ptrs, v_ptrs, slot_ids, nullptr, units, per_unit, num_units * per_unit, num_heads,
+                                num_kv_heads, head_size, q_stride, scale, max_seq_len, alibi_slopes, q_dtype, out_dtype,
+                                nullptr, 0, stream);
+  }
   if (q_dtype == VTKV_F32) {
     // float32 models: every prompt token streams its own rows through the float32 decode kernel
     VTKV_REQUIRE(kv_dtype == VTKV_F32 && out_dtype == VTKV_F32, "float32 queries take a float32 cache and a float32 result");

@@ -15,7 +15,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 import torch
 
 from .. import _C, _custom_ops as ops, vmm_allocator as vmm
-
+from .step import kv_row_bytes
 
 
 def _dtype_size(dtype: torch.dtype) -> int:
@@ -62,13 +62,21 @@ class _HostArena:
 class CacheEngine:
     def __init__(self, num_layers: int, num_kv_heads: int, head_size: int, dtype: torch.dtype, max_num_seqs: int,
                  max_num_batched_tokens: int, cache_seqs: int = 0, cache_tokens: int = 0,
-                 swap_space_bytes: int = 0, device: int = 0, value_skew: int = 256) -> None:
+                 swap_space_bytes: int = 0, device: int = 0, value_skew: int = 256,
+                 kv_cache_dtype: Optional[str] = None) -> None:
+        """``dtype``: the rows' element type (torch.uint8: an fp8 cache).  ``kv_cache_dtype="int4"``: 4-bit rows,
+        whatever ``dtype`` the model has."""
         self.num_layers = num_layers
         self.num_kv_heads = num_kv_heads
         self.head_size = head_size
         self.dtype = dtype
         self.device = device
-        self.token_size = num_kv_heads * head_size * _dtype_size(dtype)  # bytes of one K (or V) row
+        if kv_cache_dtype not in (None, "auto", "fp8", "int4"):
+            raise _C.VtkvError(_C.EINVAL, f"Unsupported data type of kv cache: {kv_cache_dtype}")
+        if kv_cache_dtype != "int4" and kv_cache_dtype is not None and (kv_cache_dtype == "fp8") != (_dtype_size(dtype) == 1):
+            raise _C.VtkvError(_C.EINVAL, f"a cache of {dtype} is not of kind {kv_cache_dtype}")
+        self.kv_cache_dtype = kv_cache_dtype or ("fp8" if _dtype_size(dtype) == 1 else "auto")
+        self.token_size = kv_row_bytes(num_kv_heads, head_size, self.kv_cache_dtype, _dtype_size(dtype))  # bytes of one K (or V) row
         # cache_engine.py:53-57: every slot reserves room for max_num_batched_tokens rows
         # (plus the bytes by which the V rows are set off from the base of their range)
         self.value_skew = int(value_skew)
@@ -86,7 +94,6 @@ class CacheEngine:
             for seg in self.vmm_kvcache_segment:
                 seg.set_value_skew(self.value_skew)
         # cache_engine.py:111-129: per layer one pointer table for K and one for V
-        self.kv_cache_dtype = "fp8" if _dtype_size(dtype) == 1 else "auto"
         self.gpu_cache = [(vmm.KV_cache(max_num_seqs, l, self.kv_cache_dtype),
                            vmm.KV_cache(max_num_seqs, l, self.kv_cache_dtype)) for l in range(num_layers)]
         vmm.copy_kv_cache([k.kv_cache for k, _ in self.gpu_cache], [v.kv_cache for _, v in self.gpu_cache],
@@ -228,8 +235,10 @@ class CacheEngine:
 
     @staticmethod
     def get_cache_block_size(block_size: int, num_kv_heads: int, head_size: int, num_layers: int,
-                             dtype: torch.dtype) -> int:
+                             dtype: torch.dtype, kv_cache_dtype: str = "auto") -> int:
         # cache_engine.py:144-162
+        if kv_cache_dtype == "int4":
+            return num_layers * 2 * block_size * kv_row_bytes(num_kv_heads, head_size, "int4")
         return _dtype_size(dtype) * num_layers * 2 * block_size * num_kv_heads * head_size
 
     def close(self) -> None:

@@ -11,8 +11,11 @@ from .. import vmm_allocator as vmm
 
 
 def kv_row_bytes(num_kv_heads: int, head_size: int, kv_cache_dtype: str = "auto", model_elem_bytes: int = 2) -> int:
-    """Bytes of one K (or V) row of one token in a sequence's range: one byte per element for an fp8 cache,
-    otherwise the model's element size (the reference hard-codes 2, llama.py:315)."""
+    """Bytes of one K (or V) row of one token in a sequence's range: one byte per element for an fp8 cache, half a
+    byte and four bytes per kv head (in steps of 16) for an int4 cache, otherwise the model's element size (the
+    reference hard-codes 2, llama.py:315)."""
+    if kv_cache_dtype == "int4":
+        return (int(num_kv_heads) * (int(head_size) // 2 + 4) + 15) // 16 * 16
     elem = 1 if kv_cache_dtype in ("fp8", "fp8_e4m3") else int(model_elem_bytes)
     return int(num_kv_heads) * int(head_size) * elem
 
@@ -23,7 +26,7 @@ def prepare_step(attn_metadata, kv_caches: Sequence, kv_cache_dtype: Optional[st
     for this step.
 
     kv_caches: per layer a (K, V) pair of ``KV_cache`` handles, or None entries during profiling.
-    kv_cache_dtype: "auto" (rows of the model's element size) or "fp8" (one byte per element); by default
+    kv_cache_dtype: "auto" (rows of the model's element size), "fp8" (one byte per element) or "int4"; by default
     what the ``CacheEngine`` that made the handles says (``KV_cache.kv_cache_dtype``), else "auto".
 
     The batch holds ``num_prefills`` prompts first, then the decode sequences (one new row each).  A prompt
@@ -140,7 +143,9 @@ class DecodeStepPlan:
         self._src_dt = ops._DTYPES[model_dtype]
         self._kv_dt = ops._kv_dtype(kv_cache_dtype, self._src_dt)
         self.k_scale, self.v_scale = float(k_scale), float(v_scale)
-        self.kv_size = self.num_kv_heads * self.head_size * {_C.FP8_E4M3: 1, _C.F32: 4}.get(self._kv_dt, 2)  # bytes per row
+        self.kv_size = kv_row_bytes(self.num_kv_heads, self.head_size, kv_cache_dtype,
+                                    4 if self._src_dt == _C.F32 else 2)  # bytes per row
+        ops._int4_scales(kv_cache_dtype, k_scale, v_scale)
         self._segments = list(segments)  # keeps the handles alive
         self._segs = (C.c_void_p * n)(*[s._h for s in segments])
         self._tok = (C.c_int64 * n)(*([self.kv_size] * n))
@@ -174,8 +179,9 @@ class DecodeStepPlan:
         self._ws = torch.zeros(max(int(need), 1 << 20), dtype=torch.uint8, device=self.device)
         self._ws_p, self._ws_n = C.c_void_p(self._ws.data_ptr()), self._ws.numel()
         self.seq_lens = None  # numpy view of the last step's lengths (valid until the ring wraps)
-        # one launch per step: any cache type at head size 128; 16-bit caches at the other head sizes
-        self.fused = bool(fused) and self._src_dt != _C.F32 and (self.head_size == 128 or self._kv_dt == self._src_dt)
+        # one launch per step: 16-bit and fp8 caches at head size 128, 16-bit caches at the other head sizes
+        self.fused = bool(fused) and self._src_dt != _C.F32 and self._kv_dt != _C.INT4 and (
+            self.head_size == 128 or self._kv_dt == self._src_dt)
         self._inline = self.fused and n <= 512
         self._host_lens_p = [C.c_void_p(self._stage[i].data_ptr() + 8 * n) for i in range(ring)]
 

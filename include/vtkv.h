@@ -34,6 +34,7 @@ extern "C" {
 #define VTKV_BF16 1
 #define VTKV_F16 2
 #define VTKV_FP8_E4M3 3 /* OCP e4m3fn, one byte per element, per-tensor scale */
+#define VTKV_INT4 4     /* 4-bit codes with a scale and a zero per token and kv head (see vtkv_kv_row_bytes) */
 
 /* copy directions for vtkv_swap_* */
 #define VTKV_D2H 0
@@ -214,12 +215,30 @@ int vtkv_memcpy_h2d_async(uint64_t dst, const void *src, int64_t bytes, void *st
  * For sequence b, token t < max_seq_len: dst = ptrs[slot_ids[b]] + slot_m[b] + t*num_heads*head_size*e_kv,
  * src row = (max_seq_len == 1) ? b : cache_seq_lens[b] + t.
  * kv_dtype == src_dtype copies bits; kv_dtype == VTKV_FP8_E4M3 stores e4m3fn(x / scale) (round to
- * nearest even, saturating at +-448), slot_m is then in bytes of the fp8 range. */
+ * nearest even, saturating at +-448), slot_m is then in bytes of the fp8 range; kv_dtype == VTKV_INT4 (bf16 and fp16
+ * sources, head sizes 64, 80, 96, 112, 128, 256) stores 4-bit rows, dst = ptrs[slot_ids[b]] + slot_m[b] +
+ * t*vtkv_kv_row_bytes(num_heads, head_size, VTKV_INT4), slot_m a multiple of 16; k_scale and v_scale are not used. */
 int vtkv_reshape_and_cache(const void *key, const void *value, const int64_t *k_ptrs, const int64_t *v_ptrs,
                            const int64_t *slot_m, const int64_t *slot_ids, const int32_t *seq_lens,
                            const int32_t *cache_seq_lens, int batch, int max_seq_len, int num_heads, int head_size,
                            int64_t key_stride, int64_t value_stride, int src_dtype, int kv_dtype, float k_scale,
                            float v_scale, void *stream);
+
+/* Bytes of one token's K (or V) row in a sequence's range, 0 for sizes that kv_dtype does not serve.  For VTKV_INT4 a
+ * row is num_kv_heads * head_size / 2 bytes of codes (value 2i of a head in the low half of its byte i), then per kv head
+ * a bfloat16 scale and a bfloat16 zero, padded to 16 bytes; a value is code * scale + zero.  zero is the smallest value of
+ * the head's row rounded to bfloat16, scale = bf16((largest - zero) / 15), code = floor((x - zero) / scale + 1/2) within
+ * 0..15.  A head's row with a value that is not finite reads back as NaN.  Row addresses are multiples of 16.  No
+ * counterpart in the reference. */
+int64_t vtkv_kv_row_bytes(int num_kv_heads, int head_size, int kv_dtype);
+
+/* The rows of a 4-bit cache back as values: the inverse of vtkv_reshape_and_cache with the same arguments, key and value
+ * receiving code * scale + zero rounded to dst_dtype (VTKV_F32, VTKV_BF16 or VTKV_F16).  kv_dtype must be VTKV_INT4.
+ * Rows with slot_m < 0, and rows behind seq_lens, are left as they were.  No counterpart in the reference. */
+int vtkv_read_cached_rows(void *key, void *value, const int64_t *k_ptrs, const int64_t *v_ptrs, const int64_t *slot_m,
+                          const int64_t *slot_ids, const int32_t *seq_lens, const int32_t *cache_seq_lens, int batch,
+                          int max_seq_len, int num_heads, int head_size, int64_t key_stride, int64_t value_stride,
+                          int dst_dtype, int kv_dtype, void *stream);
 
 /* Upstream paged scatter, the layout the reference's kernel tests pin; replaces the 7-argument
  * reshape_and_cache (csrc/cpu/cache.cpp:103-128, tests/kernels/test_cache.py:115-193).
@@ -310,7 +329,11 @@ int64_t vtkv_decode_attention_workspace_bytes(int num_seqs, int num_heads, int h
  * of its own that computes in fp32 on the vector unit; partition_tokens is ignored (partitions of 512 rows, fewer
  * rows for small batches, more where the workspace does not hold the partial results); also through
  * vtkv_decode_attention_v2, vtkv_decode_attention_noalloc and vtkv_prefill_attention (where every prompt token
- * streams its own rows: right, and quadratic in HBM traffic), not through vtkv_decode_append_attention. */
+ * streams its own rows: right, and quadratic in HBM traffic), not through vtkv_decode_append_attention.
+ * kv_dtype VTKV_INT4 (bf16 and fp16 queries, every head size and head count): a kernel of its own over 4-bit rows
+ * (see vtkv_kv_row_bytes), also through vtkv_decode_attention_noalloc and vtkv_prefill_attention, not through
+ * vtkv_decode_attention_v2 and vtkv_decode_append_attention; partition_tokens, k_scale and v_scale are not used, and a
+ * sequence of length 0 (a padded batch) gets zeros. */
 int vtkv_decode_attention(void *out, const void *q, const int64_t *k_ptrs, const int64_t *v_ptrs,
                           const int64_t *slot_ids, const int32_t *seq_lens, int num_seqs, int num_heads,
                           int num_kv_heads, int head_size, int64_t q_stride, float scale, int max_seq_len,
@@ -412,6 +435,45 @@ int vtkv_decode_append_attention(void *out, const void *q, const void *key, cons
                                  float scale, int max_seq_len, const float *alibi_slopes, int q_dtype, int out_dtype,
                                  int kv_dtype, float k_scale, float v_scale, void *workspace, int64_t workspace_bytes,
                                  int partition_tokens, void *stream);
+
+/* ------------------------------------------------------------------------------------------
+ * A cache of a bounded number of rows.  No counterpart in the reference.
+ * ---------------------------------------------------------------------------------------- */
+
+/* Adds to weights[slot, kv head, row] the attention that one query token per sequence pays to the row, summed over the
+ * kv head's query heads: sum_h softmax_row(scale * q[b,h,:] . K_b[row, kv head, :] [+ alibi]) for row < seq_lens[b].
+ *   weights    device float [num_slots, num_kv_heads, >= max_seq_len], slot_stride and head_stride in elements, rows
+ *              contiguous; indexed by slot, so that it stays with a sequence from step to step
+ *   seq_lens   device int32[num_seqs], at most max_seq_len (larger ones are cut off); 0 leaves the slot as it is
+ *   slot_ids   device int64[num_seqs]; the slots of a call are distinct, a slot outside [0, num_slots) is skipped
+ *   kv_dtype   q_dtype, VTKV_FP8_E4M3 with k_scale, or VTKV_INT4
+ *   workspace  device scratch of vtkv_accumulate_attention_weights_workspace_bytes(...) bytes, any contents
+ * Other arguments as for vtkv_decode_attention (q_dtype VTKV_BF16 or VTKV_F16).  Only K is read. */
+int64_t vtkv_accumulate_attention_weights_workspace_bytes(int num_seqs, int num_heads, int max_seq_len);
+int vtkv_accumulate_attention_weights(float *weights, int64_t slot_stride, int64_t head_stride, int64_t num_slots,
+                                      const void *q, const int64_t *k_ptrs, const int64_t *slot_ids,
+                                      const int32_t *seq_lens, int num_seqs, int num_heads, int num_kv_heads,
+                                      int head_size, int64_t q_stride, float scale, int max_seq_len,
+                                      const float *alibi_slopes, int q_dtype, int kv_dtype, float k_scale,
+                                      void *workspace, int64_t workspace_bytes, void *stream);
+
+/* Cuts every sequence of the batch that has more than keep_rows rows back to keep_rows, each kv head by itself and in
+ * place.  Of a head's n rows the last recent_rows stay, and of those before them the keep_rows - recent_rows with the
+ * largest weights[slot, kv head, row] (of equal ones the first; NaN counts as largest).  With heavy = keep_rows -
+ * recent_rows: rows below heavy that stay keep their places; the other rows that stay fill, in order, the places of the
+ * evicted ones below heavy; the recent rows move to [heavy, keep_rows) in order.  weights moves with the rows and is
+ * zero in [keep_rows, n).  new_seq_lens[b] = min(seq_lens[b], keep_rows) (may be seq_lens itself).  Rows in [keep_rows, n)
+ * of the ranges are left as they were.
+ *   seq_lens   device int32[num_seqs], at most max_seq_len; slots are distinct, one outside [0, num_slots) is skipped
+ *   kv_dtype   the rows' type: VTKV_F32, VTKV_BF16, VTKV_F16, VTKV_FP8_E4M3 or VTKV_INT4
+ *   workspace  device scratch of vtkv_evict_rows_workspace_bytes(...) bytes, any contents, 16-byte aligned
+ * The rows of a head are no longer in the order of their tokens afterwards (attention without ALiBi does not mind).  The
+ * ranges are written: chunks shared with another sequence (vtkv_seg_share_prefix) would change under it. */
+int64_t vtkv_evict_rows_workspace_bytes(int num_seqs, int num_kv_heads, int max_seq_len, int keep_rows, int recent_rows);
+int vtkv_evict_rows(const int64_t *k_ptrs, const int64_t *v_ptrs, float *weights, int64_t slot_stride,
+                    int64_t head_stride, int64_t num_slots, const int64_t *slot_ids, const int32_t *seq_lens,
+                    int32_t *new_seq_lens, int num_seqs, int num_kv_heads, int head_size, int kv_dtype, int keep_rows,
+                    int recent_rows, int max_seq_len, void *workspace, int64_t workspace_bytes, void *stream);
 
 /* Where the partial results of the workgroups that share a (sequence, kv head) are merged: 1 = inside the
  * attention kernel, by whichever of them finishes last; 0 = by a second kernel; -1 (the default) = inside

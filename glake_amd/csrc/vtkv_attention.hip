@@ -1616,8 +1616,10 @@ int64_t vtkv_decode_attention_workspace_bytes(int num_seqs, int num_heads, int h
   // (the kernels hold a head size padded to 32 elements, to 64 for fp8 rows: sized for the larger)
   // (kv heads with more than 16 query heads are served in parts that may leave some of their 16 places empty:
   // at most one sixteenth more places than heads)
-  return scratch_floats(grid, num_seqs, num_heads + num_heads / 16, (head_size + 63) / 64 * 64) * (int64_t)sizeof(float) +
-         cum_bytes + counter_bytes(num_seqs, num_heads);
+  const int64_t bytes = scratch_floats(grid, num_seqs, num_heads + num_heads / 16, (head_size + 63) / 64 * 64) *
+                            (int64_t)sizeof(float) + cum_bytes + counter_bytes(num_seqs, num_heads);
+  // (one buffer serves a 4-bit cache too)
+  return std::max(bytes, counter_bytes(0, 0) + vtkv::int4_decode_workspace_bytes(num_seqs, num_heads, head_size));
 }
 
 int vtkv_decode_attention(void *out, const void *q, const int64_t *k_ptrs, const int64_t *v_ptrs,

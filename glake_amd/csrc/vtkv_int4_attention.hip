@@ -168,7 +168,11 @@ int int4_attention(void *out, const void *q, const int64_t *k_ptrs, const int64_
   VTKV_REQUIRE(max_seq_len > 0, "max_seq_len must be > 0");
   const int group_real = num_heads / num_kv_heads, split = vtkv_kv_split(group_real);
   VTKV_REQUIRE(num_kv_heads * split <= 65535, "too many kv heads");
+  VTKV_REQUIRE(int4_row_bytes(num_kv_heads, head_size) < (4 << 20), "rows of 4 MiB and more are not supported");
   if (num_rows == 0) return VTKV_OK;
+  if (!units)
+    return int4_decode(out, q, k_ptrs, v_ptrs, slot_ids, seq_lens, num_rows, num_heads, num_kv_heads, head_size, q_stride,
+                       scale, max_seq_len, alibi_slopes, q_dtype, out_dtype, workspace, workspace_bytes, stream);
   Int4Params p;
   p.q = (const uint16_t *)q;
   p.k_ptrs = k_ptrs;

@@ -11,20 +11,21 @@
 //    eight codes and no rounding.  The other factor 16 and the 2^24 go into q, which is brought to fp16 by a power of
 //    two per head (its largest value near 2^14): exact for bf16 and fp16 queries.
 //  * V: the codes of 16 rows come out of LDS transposed (ds_read_b64_tr_b4: lane d of a group gets column d of 16
-//    rows); (word >> 4k & 0x000f000f) | 0x43004300 are the bf16 numbers 128 + c.  p s is carried as a bf16 head and a
-//    bf16 tail (2^-17 relative); the 128 sum(p s) that come with the codes are subtracted from sum(p z) in fp32, with
-//    the same head and tail, so that nothing but fp32 rounding remains of them.
+//    rows) and are masked the same way: as bf16 numbers they are c * 2^-133 and c * 2^-129, in the denormals and the
+//    binade above them, where the bits count evenly.  p s comes with a factor of 2^60 (2^56 for the rows whose codes
+//    stand 2^4 higher) and is carried as a bf16 head and a bf16 tail, both cut off (2^-15 relative).  Scales up to 2^60
+//    fit; what p s is below 2^-57 loses bits (an absolute error below 2^-53).
 //
 // How it moves data.  HBM-bound: 2 rows of 68 bytes per token and kv head (head size 128).  A workgroup takes whole
 // rows (or eight kv heads of them): a stage of 64 rows (512 / kv heads when there are fewer than eight) of K and V goes
 // from global memory straight into LDS (16 bytes per lane, no registers), two stages deep, so that loads are always in
 // flight while the other stage is computed; a row's bytes are fetched once whatever the heads per line.  Each wave
-// serves one kv head and 64 rows of the stage.
+// serves one kv head and 32 rows of the stage; sixteen waves (four per SIMD) hide each other's chains of LDS reads, MFMAs
+// and exponentials.  What the waves of a kv head hold is combined through LDS when a span's part of a sequence ends.
 //
-// Group sizes below 16 leave columns of the 16-column tiles free.  A tile's columns are (part j, head): with up to four
-// heads the four 16-row tiles of a wave's 64 rows share one tile of logits (J = 4), with up to eight in pairs (J = 2),
-// so the softmax arithmetic is per logit that exists; P.V takes the same layout with zeros where a row is not the
-// part's, and the parts are added up at the end of a span.
+// Up to eight query heads per kv head leave half of the 16-column tiles free: then a tile's columns are (part j, head)
+// and the two 16-row tiles of a wave share one tile of logits (J = 2), so the softmax arithmetic is per logit that
+// exists; P.V takes the same layout with zeros where a row is not the part's, and the parts are added up at the end.
 //
 // The batch's rows in steps of 16 are cut into as many equal spans as workgroups run; a span that ends inside a
 // sequence leaves a partial result in the workspace and a second kernel merges them.
@@ -41,12 +42,16 @@ using namespace vtkv_attn;
 
 constexpr int kMaxBatch = 1024;   // sequences per launch
 constexpr int kPtrTable = 256;    // base addresses held in LDS, of the first so many sequences
-constexpr int kTileRows = 64;     // rows of a wave's tile
+constexpr int kTileRows = 32;     // rows of a wave's tile
+constexpr int kPrivate = 512;     // LDS of a wave: the scales and zeros of its tile's K rows, then of its V rows
 constexpr int kUnitRows = 16;     // rows by which spans are cut
 constexpr int kLdsBytes = 160 * 1024;
 
-constexpr int waves_of(int d) { return d > 128 ? 4 : 8; }
-constexpr int loads_of(int d) { return d > 128 ? 9 : 5; }  // 16-byte loads per lane, stage and side at most
+constexpr int waves_of(int d) { return d > 128 ? 8 : 16; }
+constexpr int loads_of(int d) { return d > 128 ? 5 : 3; }  // 16-byte loads per lane, stage and side at most
+// blocks of 16 columns that all waves' results go through LDS at a time (what a stage of whole rows holds)
+constexpr int round_of(int d) { return d > 128 ? 8 : d / 32; }
+constexpr int results_bytes(int d) { return waves_of(d) * (round_of(d) * 1024 + 192); }
 
 struct DecodeParams {
   const uint16_t *q;
@@ -56,13 +61,13 @@ struct DecodeParams {
   void *out;
   float *part_o;    // [2 * grid][chunk heads][group][D]
   float *part_ml;   // the same without D, (maximum, sum) pairs
-  int32_t *cum;     // [num_seqs + 1] units before a sequence
+  int32_t *spans;   // [num_seqs, chunks] pairs: the place of its first partial result, the last span that holds rows of it
   int64_t q_stride;
   int num_seqs, num_heads, num_kv_heads, kv_split, group, group_real;  // (kv heads as the kernel sees them)
   int row_bytes, max_seq_len, out_f32;
   int chunk_heads, chunks, chunk_real, parts_per_real;  // kv heads of a workgroup; chunks per sequence; real kv heads of one
-  int row_tiles;               // 64-row tiles per stage
-  int stage_bytes;             // LDS of a stage: K, then V (or the results of its waves, merged when a part ends)
+  int row_tiles;               // tiles of rows per stage
+  int stage_bytes;             // LDS of a stage: K, then V (or what its waves hold, combined when a part ends)
   int code_units, scale_units; // 16-byte pieces of a row in LDS
   int min_units;               // a span's units at least
   float scale_log2;
@@ -89,14 +94,14 @@ typedef __attribute__((address_space(3))) char *lptr;
 // 16 bytes per lane from base + off to lds + 16 * lane (M0 holds lds; nothing else in these kernels uses M0).  Nothing the
 // compiler counts: the caller waits (wait_loads).
 __device__ __forceinline__ void load_to_lds(uint64_t base, uint32_t off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds), "v"(off), "s"(base) : "memory");
 }
 // Until at most n vector memory instructions are outstanding.  They retire in order, so the older ones are done.
 __device__ __forceinline__ void wait_loads(int n) {
 #define VTKV_WAIT(N)                                    \
   case N: asm volatile("s_waitcnt vmcnt(" #N ")" ::: "memory"); break;
   switch (n) {
-    VTKV_WAIT(2) VTKV_WAIT(4) VTKV_WAIT(6) VTKV_WAIT(8) VTKV_WAIT(10) VTKV_WAIT(12) VTKV_WAIT(14) VTKV_WAIT(16) VTKV_WAIT(18)
+    VTKV_WAIT(2) VTKV_WAIT(4) VTKV_WAIT(6) VTKV_WAIT(8) VTKV_WAIT(10)
     default: asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   }
 #undef VTKV_WAIT
@@ -106,47 +111,64 @@ __device__ __forceinline__ void barrier() {
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
+// x again, as a value the compiler knows nothing about: what is computed from it stays where it is used instead of being
+// kept in registers across the loop
+__device__ __forceinline__ int opaque(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+// The kernel's arguments again, for code between the loops: read from memory where they are used instead of being held in
+// scalar registers (which run out: those that do not fit are kept in vector lanes, an instruction each time) all along.
+__device__ __forceinline__ const DecodeParams &reload() {
+  auto p = (const __attribute__((address_space(4))) DecodeParams *)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const DecodeParams *)p;
+}
+__device__ __forceinline__ uint64_t uniform64(uint64_t x) {
+  return (uint64_t)(uint32_t)uniform((int)(x >> 32)) << 32 | (uint32_t)uniform((int)x);
+}
 
-// A place in the batch's order (sequence, chunk, row), with the end of the part of it that this span holds.
+// A place in the batch's order (sequence, chunk, row), with the end of the part of it that this span holds (0: past the
+// span) and the units of the span behind that part.
 struct Cursor {
-  int b, chunk, row, end, left;  // left: units of the span behind this part
-  __device__ __forceinline__ bool valid() const { return end > 0; }
+  int b, chunk, row, end, left;
 };
 
 template <int D, int J, bool F16>
 __global__ void __launch_bounds__(waves_of(D) * 64) int4_decode_kernel(DecodeParams p) {
   constexpr int kWaves = waves_of(D), kThreads = kWaves * 64, kLoads = loads_of(D);
   constexpr int kWords = D / 8, kSteps = (kWords + 3) / 4;  // words of eight codes; MFMA steps over d
-  constexpr int kDB = D / 16;
+  constexpr int kDB = D / 16, kPairs = (kDB + 1) / 2;       // blocks of 16 output columns
+  constexpr int kRound = round_of(D);
   constexpr int kHeads = 16 / J;  // columns of a part
-  constexpr int kE = 4 / J;       // tiles of logits
+  constexpr int kE = 2 / J;       // tiles of logits
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ int s_tot[kWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
-  const int g = lane >> 4, n = lane & 15;
-  const int j = n / kHeads, h = n % kHeads;  // this lane's column: part and head
+  const int n = lane & 15;
+  const int j = n / kHeads;  // this lane's column: part j, head n % kHeads
   const int B = p.num_seqs, C = p.chunks;
   const int units_row = p.code_units + p.scale_units, pitch = units_row * 16;
   const int stage_rows = p.row_tiles * kTileRows, side_bytes = stage_rows * pitch;
-  int *s_cum = reinterpret_cast<int *>(smem + 2 * p.stage_bytes);
-  uint64_t *s_ptr = reinterpret_cast<uint64_t *>(smem + 2 * p.stage_bytes + ((B + 1) * 4 + 15) / 16 * 16);
+  int *s_cum = reinterpret_cast<int *>(smem + 2 * p.stage_bytes + kWaves * kPrivate);
+  uint64_t *s_ptr = reinterpret_cast<uint64_t *>(smem + 2 * p.stage_bytes + kWaves * kPrivate + ((B + 1) * 4 + 15) / 16 * 16);
 
   // ---- units before every sequence, and the base addresses of the first ones
   {
     constexpr int kPer = (kMaxBatch + kThreads - 1) / kThreads;
     int local[kPer], sum = 0;
+    const bool in_table = tid < min(B, kPtrTable);
+    const int64_t slot = in_table ? p.slot_ids[tid] : 0;
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
       const int idx = tid * kPer + k;
       local[k] = sum;
-      if (idx < B) {
-        sum += (max(0, min(p.seq_lens[idx], p.max_seq_len)) + kUnitRows - 1) / kUnitRows;
-      }
+      if (idx < B) sum += (max(0, min(p.seq_lens[idx], p.max_seq_len)) + kUnitRows - 1) / kUnitRows;
     }
-    if (tid < min(B, kPtrTable)) {
-      const int64_t slot = p.slot_ids[tid];
+    if (in_table) {
       s_ptr[2 * tid] = (uint64_t)p.k_ptrs[slot];
       s_ptr[2 * tid + 1] = (uint64_t)p.v_ptrs[slot];
+      reinterpret_cast<int *>(s_ptr + 2 * kPtrTable)[tid] = min(p.seq_lens[tid], p.max_seq_len);
     }
     int incl = sum;
 #pragma unroll
@@ -166,8 +188,6 @@ __global__ void __launch_bounds__(waves_of(D) * 64) int4_decode_kernel(DecodePar
       if (tid * kPer + k < B) s_cum[tid * kPer + k] = excl + local[k];
     if (tid == 0) s_cum[B] = all;
     __syncthreads();
-    if (blockIdx.x == 0)
-      for (int i = tid; i <= B; i += kThreads) p.cum[i] = s_cum[i];
   }
   const int total = uniform(s_cum[B]) * C;
   const int active = active_spans(p, total, gridDim.x);
@@ -175,7 +195,11 @@ __global__ void __launch_bounds__(waves_of(D) * 64) int4_decode_kernel(DecodePar
   const int u_begin = span_begin(total, active, blockIdx.x), u_end = span_begin(total, active, blockIdx.x + 1);
   if (u_begin >= u_end) return;
 
-  auto len_of = [&](int b) { return uniform(min(p.seq_lens[b], p.max_seq_len)); };
+  auto len_of = [&](int b) {
+    if (b < kPtrTable) return uniform(reinterpret_cast<const int *>(s_ptr + 2 * kPtrTable)[b]);
+    const DecodeParams &p = reload();
+    return uniform(min(p.seq_lens[b], p.max_seq_len));
+  };
   // the part of sequence b, chunk c from unit k on, as far as `left` units go
   auto enter = [&](Cursor &c, int b, int chunk, int k, int left) {
     const int nb = uniform(s_cum[b + 1]) - uniform(s_cum[b]);
@@ -186,12 +210,12 @@ __global__ void __launch_bounds__(waves_of(D) * 64) int4_decode_kernel(DecodePar
     c.end = min(len_of(b), (k + take) * kUnitRows);
     c.left = left - take;
   };
-  auto step = [&](Cursor &c) {  // one stage on
+  auto step = [&](Cursor &c) {  // one stage on; true: into another part
     c.row += stage_rows;
-    if (c.row < c.end) return;
+    if (c.row < c.end) return false;
     if (c.left == 0) {
       c.end = 0;
-      return;
+      return true;
     }
     int b = c.b, chunk = c.chunk + 1;
     if (chunk == C) {
@@ -199,6 +223,7 @@ __global__ void __launch_bounds__(waves_of(D) * 64) int4_decode_kernel(DecodePar
       do ++b; while (uniform(s_cum[b + 1]) == uniform(s_cum[b]));  // (ends: `left` units are still to come)
     }
     enter(c, b, chunk, 0, c.left);
+    return true;
   };
   Cursor cc;
   {
@@ -206,7 +231,7 @@ __global__ void __launch_bounds__(waves_of(D) * 64) int4_decode_kernel(DecodePar
     int b = 0;
     for (int i0 = 0; i0 < B; i0 += 64) {
       const int i = i0 + lane;
-      const bool before = i < B && (int64_t)s_cum[i] * C <= u_begin && s_cum[i + 1] > s_cum[i];
+      const bool before = i < B && s_cum[i] * C <= u_begin && s_cum[i + 1] > s_cum[i];
       const unsigned long long m = __builtin_amdgcn_ballot_w64(before);
       if (m) b = i0 + 63 - __builtin_clzll(m);
     }
@@ -216,60 +241,15 @@ __global__ void __launch_bounds__(waves_of(D) * 64) int4_decode_kernel(DecodePar
     enter(cc, b, k / nb, k % nb, u_end - u_begin);
   }
 
-  // ---- stage loads: 16-byte piece i of a stage's side goes to LDS byte 16 i; lane l of load k of this wave takes
-  // piece (wave + waves * k) * 64 + l
-  const int pieces = stage_rows * units_row, num_loads = (pieces + 63) / 64;
-  int ld_row[kLoads], ld_col[kLoads];
-#pragma unroll
-  for (int k = 0; k < kLoads; ++k) {
-    const int i = (wave + kWaves * k) * 64 + lane;
-    ld_row[k] = i / units_row;
-    ld_col[k] = i % units_row;
-  }
-  const int my_loads = wave < num_loads ? (num_loads - wave + kWaves - 1) / kWaves : 0;
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(lptr)smem;
-  auto issue = [&](const Cursor &c, int buf) {
-    uint64_t kb, vb;
-    if (c.b < kPtrTable) {
-      kb = s_ptr[2 * c.b];
-      vb = s_ptr[2 * c.b + 1];
-    } else {
-      const int64_t slot = p.slot_ids[c.b];
-      kb = (uint64_t)p.k_ptrs[slot];
-      vb = (uint64_t)p.v_ptrs[slot];
-    }
-    const uint64_t from = (uint64_t)c.row * p.row_bytes;
-    kb = ((uint64_t)uniform((int)(kb >> 32)) << 32 | (uint32_t)uniform((int)kb)) + from;
-    vb = ((uint64_t)uniform((int)(vb >> 32)) << 32 | (uint32_t)uniform((int)vb)) + from;
-    const int last = min(stage_rows, c.end - c.row) - 1;  // rows past the part's end: its last row again, never used
-    const int real0 = real0_of(p, c.chunk);
-    const int code0 = p.scale_units ? real0 * (D / 2) / 16 * 16 : 0;
-    const int all_codes = p.num_kv_heads / p.kv_split * (D / 2);
-    const int scale0 = min((all_codes + 4 * real0) / 16 * 16, p.row_bytes - 16 * p.scale_units) - 16 * p.code_units;
-    const uint32_t dst = lds0 + buf * p.stage_bytes + wave * 1024;
-#pragma unroll
-    for (int k = 0; k < kLoads; ++k) {
-      if (wave + kWaves * k >= num_loads) break;
-      if ((wave + kWaves * k) * 64 + lane < pieces) {
-        const uint32_t off = min(ld_row[k], last) * p.row_bytes + ld_col[k] * 16 + (ld_col[k] < p.code_units ? code0 : scale0);
-        load_to_lds(kb, off, dst + k * kWaves * 1024);
-        load_to_lds(vb, off, dst + k * kWaves * 1024 + side_bytes);
-      }
-    }
-  };
-
   // ---- this wave's kv head and rows of the stage
   const int hs = wave % p.chunk_heads, rt = wave / p.chunk_heads;
   const bool has_tile = rt < p.row_tiles;
-  const int word0 = kWords % 4 == 0 ? g * (kWords / 4) : g * (kWords / 4) + min(g, kWords % 4);
-  const int words = kWords / 4 + (g < kWords % 4 ? 1 : 0);
-  u32x4 qop[kSteps];
-  float q_back, q_sum, slope;  // logit = s * acc * q_back + z * q_sum [+ slope * distance]
-  int k_lane, v_lane, sz_lane, head = -1, len = 0;
-  f32x4 acc[kDB];
-  float m_run, l_run, corr;
-  u32x4 raw[kSteps];
-  auto load_q = [&](const Cursor &c) {
+  // the words of a row that a lane group multiplies: the first, how many
+  auto word0_of = [](int g) { return kWords % 4 == 0 ? g * (kWords / 4) : g * (kWords / 4) + min(g, kWords % 4); };
+  auto words_of = [](int g) { return kWords / 4 + (g < kWords % 4 ? 1 : 0); };
+  auto load_q = [&](const Cursor &c, u32x4 (&raw)[kSteps]) {
+    const DecodeParams &p = reload();
+    const int lane = opaque(tid & 63), g = lane >> 4, h = lane % kHeads, word0 = word0_of(g), words = words_of(g);
     const int v = has_tile ? head_of_chunk(p, c.chunk, hs) : -1;
     const int hv = v < 0 ? 0 : heads_of(p, v), h0 = v < 0 ? 0 : first_head_of(p, v);
     const uint16_t *row = p.q + (int64_t)c.b * p.q_stride + (int64_t)(h0 + min(h, max(hv - 1, 0))) * D;
@@ -279,7 +259,68 @@ __global__ void __launch_bounds__(waves_of(D) * 64) int4_decode_kernel(DecodePar
       if (s < words && h < hv) raw[s] = *reinterpret_cast<const u32x4 *>(row + 8 * (word0 + s));
     }
   };
-  auto begin = [&](const Cursor &c) {
+
+  // ---- stage loads: 16-byte piece i of a stage's side goes to LDS byte 16 i; lane l of load k of this wave takes
+  // piece (wave + waves * k) * 64 + l
+  const int pieces = stage_rows * units_row, num_loads = (pieces + 63) / 64;
+  const int my_loads = wave < num_loads ? (num_loads - wave + kWaves - 1) / kWaves : 0;
+  int ld_row[kLoads];   // its row of the stage, and where its piece begins in a row of the cursor's chunk
+  int ld_at[kLoads];
+  uint64_t k_from, v_from;  // the cursor's first row
+  auto aim = [&](const Cursor &c) {  // at the cursor's part
+    const DecodeParams &p = reload();
+    const int real0 = real0_of(p, c.chunk);
+    const int code0 = p.scale_units ? real0 * (D / 2) / 16 * 16 : 0;
+    const int all_codes = p.num_kv_heads / p.kv_split * (D / 2);
+    const int scale0 = min((all_codes + 4 * real0) / 16 * 16, p.row_bytes - 16 * p.scale_units) - 16 * p.code_units;
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k) {
+      const int i = (wave + kWaves * k) * 64 + opaque(lane);
+      ld_row[k] = i / units_row;
+      const int col = i - ld_row[k] * units_row;
+      ld_at[k] = col * 16 + (col < p.code_units ? code0 : scale0);
+    }
+    uint64_t kb, vb;
+    if (c.b < kPtrTable) {
+      kb = s_ptr[2 * c.b];
+      vb = s_ptr[2 * c.b + 1];
+    } else {
+      const int64_t slot = p.slot_ids[c.b];
+      kb = (uint64_t)p.k_ptrs[slot];
+      vb = (uint64_t)p.v_ptrs[slot];
+    }
+    k_from = uniform64(kb) + (uint64_t)c.row * p.row_bytes;
+    v_from = uniform64(vb) + (uint64_t)c.row * p.row_bytes;
+  };
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lptr)smem + wave * 1024;
+  const uint32_t stage_step = (uint32_t)stage_rows * p.row_bytes;
+  auto issue = [&](const Cursor &c, int buf) {
+    const int last = min(stage_rows, c.end - c.row) - 1;  // rows past the part's end: its last row again, never used
+    const uint32_t dst = lds0 + buf * p.stage_bytes;
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k) {
+      if (wave + kWaves * k >= num_loads) break;
+      const uint32_t off = __umul24(min(ld_row[k], last), p.row_bytes) + ld_at[k];  // (a row is below 4 MiB)
+      if ((wave + kWaves * k) * 64 + lane < pieces) {
+        load_to_lds(k_from, off, dst + k * kWaves * 1024);
+        load_to_lds(v_from, off, dst + k * kWaves * 1024 + side_bytes);
+      }
+    }
+    k_from += stage_step;
+    v_from += stage_step;
+  };
+
+  u32x4 qop[kSteps];
+  float q_sum, slope;  // logit = (s * q_back) * acc + z * q_sum [+ slope * distance]
+  float own_mul;       // what this lane multiplies its row's scale with: q_back (K), the power of two of P.V (V)
+  int k_lane, v_lane, v_last, sz_lane, head = -1, len = 0;
+  f32x4 acc[kDB];
+  // a column's reference point, and how far a logit may be above it before it follows the maximum (-inf: no logit yet);
+  // the sums of p and of p z
+  float m_ref, lazy, l_run, z_run;
+  auto begin = [&](const Cursor &c, const u32x4 (&raw)[kSteps]) {
+    const DecodeParams &p = reload();
+    const int lane = opaque(tid & 63), g = lane >> 4, n = lane & 15, h = n % kHeads, word0 = word0_of(g);
     head = has_tile ? head_of_chunk(p, c.chunk, hs) : -1;
     len = len_of(c.b);
     float top = 0.f, sum = 0.f;
@@ -292,10 +333,12 @@ __global__ void __launch_bounds__(waves_of(D) * 64) int4_decode_kernel(DecodePar
         sum += x;
       }
     top = max_over_row_groups(top);
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
     sum = sum_over_row_groups(sum);
     const int expo = min(max((int)(__builtin_bit_cast(unsigned, top) >> 23), 14), 254);
     const float up = __builtin_bit_cast(float, (unsigned)(268 - expo) << 23);  // top * up in [2^14, 2^15)
-    q_back = (1.f / up) * 16777216.f * p.scale_log2;
+    const float q_back = (1.f / up) * 16777216.f * p.scale_log2;
     q_sum = sum * p.scale_log2;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
@@ -307,359 +350,387 @@ __global__ void __launch_bounds__(waves_of(D) * 64) int4_decode_kernel(DecodePar
         const float f = r & 1 ? 0.0625f : 1.f;
         qop[s][r] = pack_16x2<true>(x[r] * f, x[r + 4] * f);
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
+    __builtin_amdgcn_sched_barrier(0);  // (what follows must not take registers from what precedes)
     slope = 0.f;
     if (p.alibi_slopes && head >= 0 && h < heads_of(p, head)) slope = p.alibi_slopes[first_head_of(p, head) + h] * kLog2e;
-    const int real = head >= 0 ? real_kv_head(p, head) : 0;
-    const int real0 = real0_of(p, c.chunk);
+    const int real0 = real0_of(p, c.chunk), real = head >= 0 ? real_kv_head(p, head) : real0;
     const int code_at = real * (D / 2) - (p.scale_units ? real0 * (D / 2) / 16 * 16 : 0);
     const int all_codes = p.num_kv_heads / p.kv_split * (D / 2);
     const int scale_at = p.scale_units ? p.code_units * 16 + all_codes + 4 * real -
                                              min((all_codes + 4 * real0) / 16 * 16, p.row_bytes - 16 * p.scale_units)
                                        : all_codes + 4 * real;
-    // tile t's row of lane m as A operand: 16 t + 4 (m & 3) + m / 4; then a lane group's logits are rows = g mod 4,
-    // the 16 rows whose codes its lanes bring together for P.V
+    // tile t's row of lane m as A operand: 16 t + 4 (m & 3) + m / 4; then a lane group's logits are rows = g mod 4: the 8
+    // rows whose codes its lanes bring together for P.V, lanes 0..7 of the group from one block of 16 columns, lanes
+    // 8..15 from the next (the odd last block: from the same)
+    const int rt = has_tile ? wave / p.chunk_heads : 0;  // (a wave without a tile reads the first one and leaves it)
     k_lane = (rt * kTileRows + 4 * (n & 3) + (n >> 2)) * pitch + code_at + 4 * word0;
-    v_lane = side_bytes + (rt * kTileRows + 4 * n + g) * pitch + code_at;
-    sz_lane = (rt * kTileRows + 16 * j + g) * pitch + scale_at;
+    v_lane = side_bytes + (rt * kTileRows + 4 * (n & 7) + g) * pitch + code_at + 8 * (n >> 3);
+    v_last = v_lane - 8 * (n >> 3);
+    sz_lane = (lane >> 5) * side_bytes + (rt * kTileRows + 4 * (lane & 7) + (lane >> 3 & 3)) * pitch + scale_at;
 #pragma unroll
     for (int d = 0; d < kDB; ++d) acc[d] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    m_run = -INFINITY;
-    l_run = corr = 0.f;
+    // (this lane's row of the tile is 4 (lane & 7) + ..: its register of the P.V operands is odd where lane is)
+    own_mul = lane < 32 ? q_back : lane & 1 ? 0x1p56f : 0x1p60f;
+    m_ref = 0.f;
+    lazy = -INFINITY;
+    l_run = z_run = 0.f;
   };
-
-  auto compute = [&](const Cursor &c, int buf) {
-    const int rows = min(kTileRows, c.end - c.row - rt * kTileRows);
-    if (head < 0 || rows <= 0) return;
-    const char *st = smem + buf * p.stage_bytes;
-    f32x4 sa[4];
+  // what a column's value is multiplied with, for the four columns whose results this lane holds
+  auto rescale = [&](float f) {
+    const int g = opaque(lane) >> 4;
+    float a[4];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
+    for (int i = 0; i < 4; ++i) a[i] = __shfl(f, 4 * g + i);
+#pragma unroll
+    for (int d = 0; d < kDB; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[d][i] *= a[i];
+  };
+  // v_perm selector: the upper half of a float into the part's half of a register, zero into the other (12: a zero byte)
+  const unsigned half_sel = j == 0 ? 0x0c0c0302u : 0x03020c0cu;
+
+  // A tile as its wave takes it out of LDS: K codes as MFMA operands need them, V codes transposed, one (scale, zero) pair
+  // per lane.  It fits registers, so the stage's LDS is free for new loads as soon as every wave has read, not when it
+  // has computed.
+  struct Tile {
+    unsigned kw[2][kSteps], pair;
+    u32x2 vw[kPairs];
+  };
+  auto take = [&](int buf, Tile &tile) {
+    auto &kw = tile.kw;
+    const char *st = smem + buf * p.stage_bytes;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
       const char *at = st + k_lane + 16 * t * pitch;
-      unsigned w[kSteps];
       if constexpr (D == 128 || D == 256) {
 #pragma unroll
         for (int s = 0; s < kSteps; s += 4) {
           const u32x4 v = *reinterpret_cast<const u32x4 *>(at + 4 * s);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) w[s + i] = v[i];
+          for (int i = 0; i < 4; ++i) kw[t][s + i] = v[i];
         }
       } else if constexpr (D == 64) {
         const u32x2 v = *reinterpret_cast<const u32x2 *>(at);
-        w[0] = v[0];
-        w[1] = v[1];
+        kw[t][0] = v[0];
+        kw[t][1] = v[1];
       } else {
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) w[s] = *reinterpret_cast<const unsigned *>(at + 4 * s);
+        for (int s = 0; s < kSteps; ++s) kw[t][s] = *reinterpret_cast<const unsigned *>(at + 4 * s);
       }
-      sa[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    }
+    tile.pair = *reinterpret_cast<const unsigned *>(st + sz_lane);
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        const unsigned y = w[s] >> 8;
-        const u32x4 a = {w[s] & 0x000f000fu, w[s] & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u};
+    for (int dp = 0; dp < kPairs; ++dp) {
+      typedef int i32x2 __attribute__((ext_vector_type(2)));
+      tile.vw[dp] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr4_b64_v2i32((__attribute__((address_space(3))) i32x2 *)(
+                                             st + (kDB % 2 == 1 && 2 * dp + 1 == kDB ? v_last : v_lane) + 16 * dp)));
+    }
+  };
+  auto compute = [&](const Cursor &c, const Tile &tile) {
+    const int rows = min(kTileRows, c.end - c.row - rt * kTileRows);
+    if (head < 0 || rows <= 0) return;
+    f32x4 sa[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) sa[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const unsigned w = tile.kw[t][s], y = w >> 8;
+        const u32x4 a = {w & 0x000f000fu, w & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u};
         sa[t] = mfma_16x16x32<true>(a, qop[s], sa[t]);
       }
+    // The scales and zeros change lanes through the wave's own LDS (whose operations keep their order): row 16 t + 4 i + g
+    // is held by lane 8 g + 4 t + i (K), 32 lanes on (V); each lane prepares its row's for all columns.
+    const int at_lane = opaque(lane);
+    char *own = smem + 2 * p.stage_bytes + wave * kPrivate;
+    {
+      float *at = reinterpret_cast<float *>(own + 8 * (at_lane & 32) + 4 * (at_lane & 31));
+      at[0] = __builtin_bit_cast(float, tile.pair << 16) * own_mul;
+      at[32] = __builtin_bit_cast(float, tile.pair & 0xffff0000u);
     }
-    // x[e][i]: the lane's logit of row 16 (J e + j) + 4 i + g
-    float x[kE][4];
-    if constexpr (J == 4) {
+    own += 32 * (at_lane >> 4) + (J == 2 ? 16 * (at_lane >> 3 & 1) : 0);
+    f32x4 k_s[kE], k_z[kE], v_s[kE], v_z[kE];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[0][i] = j < 2 ? (j == 0 ? sa[0][i] : sa[1][i]) : (j == 2 ? sa[2][i] : sa[3][i]);
-    } else if constexpr (J == 2) {
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[e][i] = j == 0 ? sa[2 * e][i] : sa[2 * e + 1][i];
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[e][i] = sa[e][i];
+    for (int e = 0; e < kE; ++e) {
+      k_s[e] = *reinterpret_cast<const f32x4 *>(own + 16 * e);
+      k_z[e] = *reinterpret_cast<const f32x4 *>(own + 128 + 16 * e);
     }
-    const float ahead = (float)(c.row + rt * kTileRows + 16 * j + g - len + 1);
-    float top = -INFINITY;
+    auto values = [&]() {
+#pragma unroll
+      for (int e = 0; e < kE; ++e) {
+        v_s[e] = *reinterpret_cast<const f32x4 *>(own + 256 + 16 * e);
+        v_z[e] = *reinterpret_cast<const f32x4 *>(own + 384 + 16 * e);
+      }
+    };
+    if constexpr (J == 2) values();
+    __builtin_amdgcn_sched_barrier(0);
+    // x[e][i]: how far the lane's logit of row 16 (J e + j) + 4 i + g is above the reference point
+    float x[kE][4], a[kE][4], top = -INFINITY;
 #pragma unroll
     for (int e = 0; e < kE; ++e)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const unsigned sz = *reinterpret_cast<const unsigned *>(st + sz_lane + (16 * J * e + 4 * i) * pitch);
-        const float s = __builtin_bit_cast(float, sz << 16), z = __builtin_bit_cast(float, sz & 0xffff0000u);
-        x[e][i] = __builtin_fmaf(s * x[e][i], q_back, z * q_sum) + slope * (ahead + (float)(16 * J * e + 4 * i));
-      }
-    if (rows < kTileRows) {
+      for (int i = 0; i < 4; ++i) a[e][i] = J == 2 ? (j == 0 ? sa[0][i] : sa[1][i]) : sa[e][i];
+    auto logits = [&]() {
 #pragma unroll
       for (int e = 0; e < kE; ++e)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (16 * (J * e + j) + 4 * i + g >= rows) x[e][i] = -INFINITY;
-    }
+          x[e][i] = __builtin_fmaf(k_s[e][i], a[e][i], __builtin_fmaf(k_z[e][i], q_sum, -m_ref));
+      if (p.alibi_slopes) {
+        const float ahead = (float)(c.row + rt * kTileRows + 16 * (J == 2 ? at_lane >> 3 & 1 : 0) + (at_lane >> 4) - len + 1);
 #pragma unroll
-    for (int e = 0; e < kE; ++e)
+        for (int e = 0; e < kE; ++e)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) top = fmaxf(top, x[e][i]);
-    // the reference point of a column follows its maximum only when that has grown by more than 8 (a factor 256 in
-    // the weights): the rescale of the accumulators becomes rare
-    if (__builtin_amdgcn_ballot_w64(top > m_run + 8.f) != 0) {
+          for (int i = 0; i < 4; ++i) x[e][i] = __builtin_fmaf(slope, ahead + (float)(16 * J * e + 4 * i), x[e][i]);
+      }
+      if (rows < kTileRows) {
+        const int row = 16 * (J == 2 ? at_lane >> 3 & 1 : 0) + (at_lane >> 4);
+#pragma unroll
+        for (int e = 0; e < kE; ++e)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (16 * J * e + 4 * i + row >= rows) x[e][i] = -INFINITY;
+      }
+      top = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < kE; ++e)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, x[e][i]);
+    };
+    logits();
+    // The reference point of a column follows its maximum only when that has grown by more than 8 (a factor 256 in
+    // the weights): the rescale of the accumulators becomes rare.
+    if (__builtin_amdgcn_ballot_w64(top > lazy) != 0) {
       const float t = max_over_row_groups(top);
-      const float m_new = t > m_run + 8.f ? t : m_run;
-      const float alpha = m_new == m_run ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
-      m_run = m_new;
+      const bool moves = t > lazy;  // (its first logit, where lazy is -inf)
+      const float alpha = moves ? (lazy == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(-t)) : 1.f;
+      if (moves) {
+        m_ref += t;
+        lazy = 8.f;
+      }
       l_run *= alpha;
-      corr *= alpha;
-      float a[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) a[i] = __shfl(alpha, 4 * g + i);
-#pragma unroll
-      for (int d = 0; d < kDB; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[d][i] *= a[i];
+      z_run *= alpha;
+      rescale(alpha);
+      logits();
     }
-    const float m_ref = m_run == -INFINITY ? 0.f : m_run;  // (nothing but masked rows so far)
-    // heads and tails of p * s as A operands of P.V: word w's register r holds rows r and r + 4 of its eight
-    u32x4 ph[2], pt[2];
-#pragma unroll
-    for (int w = 0; w < 2; ++w) ph[w] = pt[w] = (u32x4){0, 0, 0, 0};
-    float ps_sum = 0.f;
+    if constexpr (J == 1) {  // (twice the logits: registers are short until they are done)
+      __builtin_amdgcn_sched_barrier(0);
+      values();
+    }
+    // heads and tails of p * s as A operands of P.V: register r holds rows r and r + 4 of the group's eight (J = 2: the
+    // lane's half of it, the other zero).  Both are cut off after 8 bits: the tail takes what the head leaves.
+    u32x4 ph, pt;
+    float ps[kE][4], rest[kE][4];
 #pragma unroll
     for (int e = 0; e < kE; ++e)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const unsigned sz = *reinterpret_cast<const unsigned *>(st + side_bytes + sz_lane + (16 * J * e + 4 * i) * pitch);
-        const float s = __builtin_bit_cast(float, sz << 16), z = __builtin_bit_cast(float, sz & 0xffff0000u);
-        const float pr = __builtin_amdgcn_exp2f(x[e][i] - m_ref);
+        const float pr = __builtin_amdgcn_exp2f(x[e][i]);
         l_run += pr;
-        corr = __builtin_fmaf(pr, z, corr);
-        const float ps = pr * s;
-        const unsigned hi = vtkv::f32_to_bf16_bits_rne(ps);
-        const float hf = __builtin_bit_cast(float, hi << 16);
-        const unsigned lo = vtkv::f32_to_bf16_bits_rne(ps - hf);
-        ps_sum += hf + __builtin_bit_cast(float, lo << 16);
-        if constexpr (J == 1) {
-          ph[e >> 1][i] |= e & 1 ? hi << 16 : hi;
-          pt[e >> 1][i] |= e & 1 ? lo << 16 : lo;
-        } else if constexpr (J == 2) {
-          ph[e][i] = j ? hi << 16 : hi;
-          pt[e][i] = j ? lo << 16 : lo;
-        } else {
-          const unsigned a = j & 1 ? hi << 16 : hi, b = j & 1 ? lo << 16 : lo;
-          ph[0][i] = j < 2 ? a : 0u;
-          pt[0][i] = j < 2 ? b : 0u;
-          ph[1][i] = j < 2 ? 0u : a;
-          pt[1][i] = j < 2 ? 0u : b;
-        }
+        z_run = __builtin_fmaf(pr, v_z[e][i], z_run);
+        ps[e][i] = pr * v_s[e][i];
+        rest[e][i] = ps[e][i] - __builtin_bit_cast(float, __builtin_bit_cast(unsigned, ps[e][i]) & 0xffff0000u);
       }
-    corr = __builtin_fmaf(-128.f, ps_sum, corr);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (J == 1) {
+        ph[i] = __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, ps[1][i]), __builtin_bit_cast(unsigned, ps[0][i]), 0x07060302u);
+        pt[i] = __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, rest[1][i]), __builtin_bit_cast(unsigned, rest[0][i]), 0x07060302u);
+      } else {
+        ph[i] = __builtin_amdgcn_perm(0u, __builtin_bit_cast(unsigned, ps[0][i]), half_sel);
+        pt[i] = __builtin_amdgcn_perm(0u, __builtin_bit_cast(unsigned, rest[0][i]), half_sel);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int d = 0; d < kDB; ++d) {
-      typedef int i32x2 __attribute__((ext_vector_type(2)));
-      const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr4_b64_v2i32(
-                                                    (__attribute__((address_space(3))) i32x2 *)(st + v_lane + 8 * d)));
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        u32x4 b;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) b[r] = ((w[k] >> (4 * r)) & 0x000f000fu) | 0x43004300u;
-        acc[d] = mfma_16x16x32<false>(ph[k], b, acc[d]);
-        acc[d] = mfma_16x16x32<false>(pt[k], b, acc[d]);
-      }
+      const unsigned w = tile.vw[d / 2][d & 1], y = w >> 8;
+      const u32x4 b = {w & 0x000f000fu, w & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u};
+      acc[d] = mfma_16x16x32<false>(ph, b, acc[d]);
+      acc[d] = mfma_16x16x32<false>(pt, b, acc[d]);
     }
   };
 
-  // ---- the end of a part: o and the statistics over the row groups and the parts of a column
-  auto fold = [&](float &m_tot, float &l_tot, float &c_tot) {
-    const float l = sum_over_row_groups(l_run), c = sum_over_row_groups(corr);
-    m_tot = m_run;
-    if constexpr (J >= 2) m_tot = fmaxf(m_tot, __shfl_xor(m_tot, 8));
-    if constexpr (J >= 4) m_tot = fmaxf(m_tot, __shfl_xor(m_tot, 4));
-    const float f = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run - m_tot);
-    l_tot = l * f;
-    c_tot = c * f;
-    if constexpr (J >= 2) l_tot += __shfl_xor(l_tot, 8), c_tot += __shfl_xor(c_tot, 8);
-    if constexpr (J >= 4) l_tot += __shfl_xor(l_tot, 4), c_tot += __shfl_xor(c_tot, 4);
-    if constexpr (J > 1) {
-      float a[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) a[i] = __shfl(f, 4 * g + i);
+  // ---- the end of a part: what the waves of a kv head hold (row tiles, and the parts of a column) is added up through
+  // the stage that has been used up, some blocks of columns at a time, and stored: the result, or this span's share of one
+  auto finish = [&](const Cursor &c, int first_row, bool first_part, int buf) {
+    const DecodeParams &p = reload();
+    const int tid = opaque(threadIdx.x), lane = tid & 63, g = lane >> 4, n = lane & 15;
+    l_run = sum_over_row_groups(l_run);
+    z_run = sum_over_row_groups(z_run);
+    float *so = reinterpret_cast<float *>(smem + buf * p.stage_bytes), *sml = so + kWaves * kRound * 256;
+    if (g == 0) {
+      sml[(wave * 16 + n) * 3] = lazy == -INFINITY ? -INFINITY : m_ref;
+      sml[(wave * 16 + n) * 3 + 1] = l_run;
+      sml[(wave * 16 + n) * 3 + 2] = z_run;
+    }
+    const bool whole = first_row == 0 && c.end == len;
+    const int place = 2 * (int)blockIdx.x + (first_part ? 0 : 1);
+    if (tid == 0) {
+      int32_t *span = p.spans + 2 * ((int64_t)c.b * C + c.chunk);
+      if (first_row == 0) span[0] = place;
+      if (c.end == len) span[1] = blockIdx.x;
+    }
+#pragma unroll 1
+    for (int d0 = 0; d0 < kDB; d0 += kRound) {
 #pragma unroll
       for (int d = 0; d < kDB; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float v = acc[d][i] * a[i], v0, v1;
-          if constexpr (J == 4) {
-            v = sum_over_row_groups(v);
-          } else {
-            swap_rows32(v, v0, v1);
-            v = v0 + v1;
-          }
-          acc[d][i] = v;
-        }
-    }
-  };
-  // the head whose results a lane holds in place i, and whether this lane stores block d of it
-  auto head_at = [&](int i) { return J == 4 ? i : J == 2 ? 4 * (g & 1) + i : 4 * g + i; };
-  auto stores = [&](int d) { return J == 4 ? (d & 3) == g : J == 2 ? (d & 1) == (g >> 1) : true; };
-  // which result a part gives: -1: the sequence's own, whole; else its place among the partial ones
-  auto place_of = [&](const Cursor &c, int first_row, bool first_part) {
-    return first_row == 0 && c.end == len ? -1 : 2 * (int)blockIdx.x + (first_part ? 0 : 1);
-  };
-  auto put = [&](const Cursor &c, int v, int hh, int d, float o, float l) {  // one value of head hh of kv head v
-    const int64_t at = ((int64_t)c.b * p.num_heads + first_head_of(p, v) + hh) * D + d;
-    const float r = o / l;
-    if (p.out_f32) reinterpret_cast<float *>(p.out)[at] = r;
-    else reinterpret_cast<uint16_t *>(p.out)[at] = f32_to_16<F16>(r);
-  };
-  auto finish = [&](const Cursor &c, int first_row, bool first_part, int buf) {
-    const int place = place_of(c, first_row, first_part);
-    float m_tot, l_tot, c_tot;
-    fold(m_tot, l_tot, c_tot);
-    const int hv = head >= 0 ? heads_of(p, head) : 0;
-    if (p.row_tiles == 1) {
-      float lh[4], ch[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        lh[i] = __shfl(l_tot, head_at(i));
-        ch[i] = __shfl(c_tot, head_at(i));
-      }
-      const int64_t base = ((int64_t)place * p.chunk_heads + hs) * p.group;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int hh = head_at(i);
-        if (hh >= hv) continue;
-#pragma unroll
-        for (int d = 0; d < kDB; ++d) {
-          if (!stores(d)) continue;
-          const float o = acc[d][i] + ch[i];
-          if (place < 0) put(c, head, hh, 16 * d + n, o, lh[i]);
-          else p.part_o[(base + hh) * D + 16 * d + n] = o;
-        }
-      }
-      if (place >= 0 && g == 0 && n < kHeads && n < hv) {
-        p.part_ml[(base + n) * 2] = m_tot;
-        p.part_ml[(base + n) * 2 + 1] = l_tot;
-      }
-    } else {
-      // several waves hold rows of one kv head: through the stage that has just been used up
-      float *so = reinterpret_cast<float *>(smem + buf * p.stage_bytes);
-      float *sml = so + p.chunk_heads * p.row_tiles * kHeads * D;
-      float ch[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) ch[i] = __shfl(c_tot, head_at(i));
-      if (has_tile) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int d = 0; d < kDB; ++d)
-            if (stores(d)) so[(wave * kHeads + head_at(i)) * D + 16 * d + n] = acc[d][i] + ch[i];
-        if (g == 0 && n < kHeads) {
-          sml[(wave * kHeads + n) * 2] = m_tot;
-          sml[(wave * kHeads + n) * 2 + 1] = l_tot;
-        }
-      }
+        if (d / kRound * kRound == d0)
+          *reinterpret_cast<f32x4 *>(so + (wave * kRound + d % kRound) * 256 + lane * 4) = acc[d];
       barrier();
-      for (int idx = tid; idx < p.chunk_heads * kHeads * D; idx += kThreads) {
-        const int d = idx % D, hh = idx / D % kHeads, place_h = idx / (D * kHeads);
-        const int v = head_of_chunk(p, c.chunk, place_h);
-        if (v < 0 || hh >= heads_of(p, v)) continue;
-        float m = -INFINITY, l = 0.f, o = 0.f;
-        for (int r = 0; r < p.row_tiles; ++r) m = fmaxf(m, sml[((r * p.chunk_heads + place_h) * kHeads + hh) * 2]);
-        for (int r = 0; r < p.row_tiles; ++r) {
-          const int w = (r * p.chunk_heads + place_h) * kHeads + hh;
-          const float f = sml[w * 2] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sml[w * 2] - m);
-          l += sml[w * 2 + 1] * f;
-          o += so[w * D + d] * f;
-        }
-        const int64_t base = ((int64_t)place * p.chunk_heads + place_h) * p.group + hh;
-        if (place < 0) {
-          put(c, v, hh, d, o, l);
-        } else {
-          p.part_o[base * D + d] = o;
-          if (d == 0) {
-            p.part_ml[base * 2] = m;
-            p.part_ml[base * 2 + 1] = l;
+      // one thread: four neighbouring columns of one query head
+      const int quads = min(kRound, kDB - d0) * 4;
+#pragma unroll 1
+      for (int idx = tid; idx < p.chunk_heads * kHeads * kRound * 4; idx += kThreads) {
+        const int dq = idx % (kRound * 4), hh = idx / (kRound * 4) % kHeads, at_hs = idx / (kRound * 4) / kHeads;
+        const int v = head_of_chunk(p, c.chunk, at_hs);
+        if (dq >= quads || v < 0 || hh >= heads_of(p, v)) continue;
+        float m = -INFINITY, l = 0.f, cr = 0.f;
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+        for (int w = at_hs; w < p.row_tiles * p.chunk_heads; w += p.chunk_heads)
+#pragma unroll
+          for (int jj = 0; jj < J; ++jj) m = fmaxf(m, sml[(w * 16 + jj * kHeads + hh) * 3]);
+        for (int w = at_hs; w < p.row_tiles * p.chunk_heads; w += p.chunk_heads)
+#pragma unroll
+          for (int jj = 0; jj < J; ++jj) {
+            const int col = jj * kHeads + hh;  // of P; the row of P.V's result
+            const float *ml = sml + (w * 16 + col) * 3;
+            const float f = ml[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[0] - m);
+            l += ml[1] * f;
+            cr += ml[2] * f;
+            const float *from = so + (w * kRound + dq / 4) * 256 + (col / 4 * 16 + dq % 4 * 4) * 4 + col % 4;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = __builtin_fmaf(from[4 * i] * 0x1p73f, f, o[i]);  // (133 - 60 binades)
           }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] += cr;
+        const int d = 16 * d0 + 4 * dq;
+        if (whole) {
+          const int64_t at = ((int64_t)c.b * p.num_heads + first_head_of(p, v) + hh) * D + d;
+          const float r = 1.f / l;
+          if (p.out_f32)
+            *reinterpret_cast<f32x4 *>(reinterpret_cast<float *>(p.out) + at) = o * r;
+          else
+            *reinterpret_cast<u32x2 *>(reinterpret_cast<uint16_t *>(p.out) + at) =
+                (u32x2){pack_16x2<F16>(o[0] * r, o[1] * r), pack_16x2<F16>(o[2] * r, o[3] * r)};
+        } else {
+          const int64_t at = ((int64_t)place * p.chunk_heads + at_hs) * p.group + hh;
+          *reinterpret_cast<f32x4 *>(p.part_o + at * D + d) = o;
+          if (d == 0) *reinterpret_cast<u32x2 *>(p.part_ml + at * 2) = (u32x2){__builtin_bit_cast(unsigned, m), __builtin_bit_cast(unsigned, l)};
         }
       }
       barrier();
     }
   };
 
-  // ---- the pipeline: while stage s is computed, stage s + 1 is on its way
-  Cursor lc = cc;
-  load_q(cc);
-  begin(cc);
-  issue(lc, 0);
-  step(lc);
-  bool more = lc.valid();
-  if (more) {
-    issue(lc, 1);
-    step(lc);
-  }
-  int first_row = cc.row;
-  bool first_part = true;
+  // ---- the pipeline: while a stage is computed, the next one is on its way
+  Cursor lc = cc, now = cc;
+  int ahead = 0, first_row = cc.row;  // stages asked for and not yet computed
+  bool fresh = true, first_part = true, any = false, aimed = false;
+  auto ask = [&](int next) {  // for two stages from the one that is computed next on
+    for (; ahead < 2 && lc.end > 0; ++ahead) {
+      if (!aimed) aim(lc);
+      issue(lc, next ^ ahead);
+      aimed = !step(lc);
+    }
+  };
   for (int buf = 0;; buf ^= 1) {
-    wait_loads(more ? 2 * my_loads : 0);
-    barrier();
-    const Cursor now = cc;
-    step(cc);
-    const bool part_ends = now.row + stage_rows >= now.end;
-    if (part_ends && cc.valid()) load_q(cc);
-    compute(now, buf);
-    barrier();
-    if (part_ends) {
-      finish(now, first_row, first_part, buf);
-      if (!cc.valid()) return;
-      first_part = false;
-      begin(cc);
-      first_row = cc.row;
+    if (fresh) {  // between two parts (before new loads are asked for: the wait for q would be a wait for them, too)
+      u32x4 raw[kSteps] = {};
+      if (cc.end > 0) load_q(cc, raw);
+      if (any) {
+        finish(now, first_row, first_part, buf ^ 1);
+        if (cc.end == 0) return;
+        first_part = false;
+        first_row = cc.row;
+      }
+      begin(cc, raw);
     }
-    more = lc.valid();
-    if (more) {
-      issue(lc, buf);
-      step(lc);
-    }
+    ask(buf);
+    wait_loads(ahead == 2 ? 2 * my_loads : 0);
+    barrier();
+    now = cc;
+    fresh = step(cc);
+    Tile tile;
+    take(buf, tile);
+    barrier();
+    --ahead;
+    // (the last stage of a part is left to its results)
+    if (!fresh) ask(buf ^ 1);
+    compute(now, tile);
+    any = true;
   }
 }
 
-// Merges the partial results of a (sequence, query head); writes zeros where there are no rows.
+// Merges the partial results of a (sequence, query head); writes zeros where there are no rows.  The partial results are
+// dealt to groups of D / 4 lanes with four values each.
 template <int D, bool F16>
-__global__ void __launch_bounds__(256) int4_merge_kernel(DecodeParams p, int grid) {
-  const int v = blockIdx.y, b = blockIdx.x, C = p.chunks;
-  const int hv = heads_of(p, v), h0 = first_head_of(p, v);
-  const int c0 = p.cum[b], nb = p.cum[b + 1] - c0, total = p.cum[p.num_seqs] * C;
-  int chunk, hs;
-  if (p.kv_split == 1) {
-    chunk = v / p.chunk_heads;
-    hs = v % p.chunk_heads;
-  } else {
-    const int part = v % p.kv_split;
-    chunk = v / p.kv_split * p.parts_per_real + part / p.chunk_heads;
+__global__ void __launch_bounds__(256) int4_merge_kernel(DecodeParams p) {
+  constexpr int kLanes = D / 4, kGroups = 256 / kLanes, kUnroll = 4;
+  __shared__ float s_o[kGroups][D], s_m[kGroups], s_l[kGroups];
+  const int b = blockIdx.x, head = blockIdx.y;
+  const int real = head / p.group_real, in_real = head % p.group_real;
+  int hh = in_real, hs = real % p.chunk_heads, chunk = real / p.chunk_heads;
+  if (p.kv_split > 1) {
+    const int part = in_real / p.group;
+    hh = in_real % p.group;
     hs = part % p.chunk_heads;
+    chunk = real * p.parts_per_real + part / p.chunk_heads;
   }
-  const int active = total ? active_spans(p, total, grid) : 1;
-  const int u0 = c0 * C + chunk * nb, u1 = u0 + nb;
-  // span of unit u: the last i with total * i / active <= u
-  auto span_of = [&](int u) {
-    int i = (int)(((int64_t)u * active) / total);
-    while (i + 1 < active && span_begin(total, active, i + 1) <= u) ++i;
-    return i;
-  };
-  const int i0 = nb ? span_of(u0) : 0, i1 = nb ? span_of(u1 - 1) : 0;
-  if (nb && i0 == i1) return;
-  for (int idx = threadIdx.x; idx < hv * D; idx += 256) {
-    const int hh = idx / D, d = idx % D;
-    float m = -INFINITY, l = 0.f, o = 0.f;
-    for (int i = i0; nb && i <= i1; ++i) {
-      const int place = 2 * i + (span_begin(total, active, i) >= u0 ? 0 : 1);
+  const int len = min(p.seq_lens[b], p.max_seq_len);
+  const int32_t *span = p.spans + 2 * ((int64_t)b * p.chunks + chunk);
+  const int first = len > 0 ? span[0] : 0, i0 = first / 2, i1 = len > 0 ? span[1] : -1;
+  if (i0 == i1) return;
+  const int grp = threadIdx.x / kLanes, d = threadIdx.x % kLanes * 4;
+  float m = -INFINITY, l = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int i = i0 + grp; grp < kGroups && i <= i1; i += kGroups * kUnroll) {
+    float mi[kUnroll], li[kUnroll];
+    f32x4 oi[kUnroll];
+#pragma unroll
+    for (int k = 0; k < kUnroll; ++k) {
+      const int at = min(i + k * kGroups, i1);
+      const int place = at == i0 ? first : 2 * at;
       const int64_t base = ((int64_t)place * p.chunk_heads + hs) * p.group + hh;
-      const float mi = p.part_ml[base * 2], li = p.part_ml[base * 2 + 1], oi = p.part_o[base * D + d];
-      const float mn = fmaxf(m, mi);
-      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn), fi = mi == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mi - mn);
-      l = l * f + li * fi;
-      o = o * f + oi * fi;
-      m = mn;
+      mi[k] = i + k * kGroups <= i1 ? p.part_ml[base * 2] : -INFINITY;
+      li[k] = p.part_ml[base * 2 + 1];
+      oi[k] = *reinterpret_cast<const f32x4 *>(p.part_o + base * D + d);
     }
-    const float r = nb ? o / l : 0.f;
-    const int64_t at = ((int64_t)b * p.num_heads + h0 + hh) * D + d;
+    float mn = m;
+#pragma unroll
+    for (int k = 0; k < kUnroll; ++k) mn = fmaxf(mn, mi[k]);
+    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+    l *= f;
+    o *= f;
+#pragma unroll
+    for (int k = 0; k < kUnroll; ++k) {
+      const float fi = mi[k] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mi[k] - mn);
+      l += li[k] * fi;
+      o += oi[k] * fi;
+    }
+    m = mn;
+  }
+  if (grp < kGroups) {
+    *reinterpret_cast<f32x4 *>(&s_o[grp][d]) = o;
+    if (d == 0) {
+      s_m[grp] = m;
+      s_l[grp] = l;
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x < D) {
+    float mm = -INFINITY, ll = 0.f, oo = 0.f;
+    for (int k = 0; k < kGroups; ++k) mm = fmaxf(mm, s_m[k]);
+    for (int k = 0; k < kGroups; ++k) {
+      const float f = s_m[k] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[k] - mm);
+      ll += s_l[k] * f;
+      oo += s_o[k][threadIdx.x] * f;
+    }
+    const float r = len > 0 ? oo / ll : 0.f;
+    const int64_t at = ((int64_t)b * p.num_heads + head) * D + threadIdx.x;
     if (p.out_f32) reinterpret_cast<float *>(p.out)[at] = r;
     else reinterpret_cast<uint16_t *>(p.out)[at] = f32_to_16<F16>(r);
   }
@@ -668,16 +739,14 @@ __global__ void __launch_bounds__(256) int4_merge_kernel(DecodeParams p, int gri
 template <int D>
 int launch_decode(const DecodeParams &p, int j, bool f16, int grid, size_t lds, hipStream_t st) {
   typedef void (*Kernel)(DecodeParams);
-  static const Kernel kernels[2][3] = {
-      {int4_decode_kernel<D, 1, false>, int4_decode_kernel<D, 2, false>, int4_decode_kernel<D, 4, false>},
-      {int4_decode_kernel<D, 1, true>, int4_decode_kernel<D, 2, true>, int4_decode_kernel<D, 4, true>}};
-  Kernel k = kernels[f16][j == 4 ? 2 : j == 2 ? 1 : 0];
-  hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(waves_of(D) * 64), lds, st, p);
-  const dim3 mg((unsigned)p.num_seqs, (unsigned)p.num_kv_heads);
+  static const Kernel kernels[2][2] = {{int4_decode_kernel<D, 1, false>, int4_decode_kernel<D, 2, false>},
+                                       {int4_decode_kernel<D, 1, true>, int4_decode_kernel<D, 2, true>}};
+  hipLaunchKernelGGL(kernels[f16][j == 2], dim3((unsigned)grid), dim3(waves_of(D) * 64), lds, st, p);
+  const dim3 mg((unsigned)p.num_seqs, (unsigned)p.num_heads);
   if (f16)
-    hipLaunchKernelGGL((int4_merge_kernel<D, true>), mg, dim3(256), 0, st, p, grid);
+    hipLaunchKernelGGL((int4_merge_kernel<D, true>), mg, dim3(256), 0, st, p);
   else
-    hipLaunchKernelGGL((int4_merge_kernel<D, false>), mg, dim3(256), 0, st, p, grid);
+    hipLaunchKernelGGL((int4_merge_kernel<D, false>), mg, dim3(256), 0, st, p);
   VTKV_HIP(hipGetLastError());
   return VTKV_OK;
 }
@@ -685,10 +754,10 @@ int launch_decode(const DecodeParams &p, int j, bool f16, int grid, size_t lds, 
 int round_up(int x, int m) { return (x + m - 1) / m * m; }
 
 // The shape of a launch: kv heads and row tiles per workgroup, its LDS.
-int plan(DecodeParams &p, int d, int kv_real, int j, size_t &lds) {
-  const int waves = waves_of(d);
+int plan(DecodeParams &p, int d, int kv_real, size_t &lds) {
+  const int waves = waves_of(d), most = waves / 2;  // (at least two row tiles: 64 rows of a stage)
   if (p.kv_split == 1) {
-    int hc = waves;
+    int hc = most;
     while (kv_real % hc) hc /= 2;
     p.chunk_heads = hc;
     p.chunk_real = hc;
@@ -696,7 +765,7 @@ int plan(DecodeParams &p, int d, int kv_real, int j, size_t &lds) {
     p.parts_per_real = 1;
   } else {
     int hc = 1;
-    while (hc < p.kv_split && hc < waves) hc *= 2;
+    while (hc < p.kv_split && hc < most) hc *= 2;
     p.chunk_heads = hc;
     p.chunk_real = 1;
     p.parts_per_real = (p.kv_split + hc - 1) / hc;
@@ -712,18 +781,17 @@ int plan(DecodeParams &p, int d, int kv_real, int j, size_t &lds) {
                              p.row_bytes / 16);
   }
   const int pitch = (p.code_units + p.scale_units) * 16;
-  const int extra = round_up((p.num_seqs + 1) * 4, 16) + std::min(p.num_seqs, kPtrTable) * 16;
+  const int extra = waves * kPrivate + round_up((p.num_seqs + 1) * 4, 16) + kPtrTable * 20;
   p.row_tiles = waves / p.chunk_heads;
   for (;; --p.row_tiles) {
-    // (a tile's results need less than its rows where every kv head has rows of its own, more where several parts of a
-    // kv head read the same ones)
-    const int results = p.row_tiles > 1 ? p.row_tiles * p.chunk_heads * (16 / j) * (4 * d + 8) : 0;
-    p.stage_bytes = round_up(std::max(2 * p.row_tiles * kTileRows * pitch, results), 16);
+    // (the results of a round need less than the rows where every kv head has rows of its own, more where several parts
+    // of a kv head read the same ones)
+    p.stage_bytes = round_up(std::max(2 * p.row_tiles * kTileRows * pitch, results_bytes(d)), 16);
     lds = (size_t)2 * p.stage_bytes + extra;
-    if (lds + 256 <= kLdsBytes && p.row_tiles * pitch / 16 <= loads_of(d) * waves) break;
+    if (lds + 256 <= kLdsBytes && (p.row_tiles * kTileRows * pitch / 16 + 63) / 64 <= loads_of(d) * waves) break;
     VTKV_REQUIRE(p.row_tiles > 1, "rows of %d bytes leave no room for a stage", p.row_bytes);
   }
-  p.min_units = 2 + 2 * p.row_tiles;
+  p.min_units = std::max(4, p.row_tiles);
   return VTKV_OK;
 }
 
@@ -733,7 +801,7 @@ namespace vtkv {
 
 int64_t int4_decode_workspace_bytes(int num_seqs, int num_heads, int head_size) {
   const int64_t heads = std::min<int64_t>(128, num_heads + num_heads / 16 + 16);
-  return 2ll * kDecodeSpans * heads * (head_size + 2) * 4 + ((int64_t)std::min(num_seqs, kMaxBatch) + 1) * 4 + 64;
+  return 2ll * kDecodeSpans * heads * (head_size + 2) * 4 + (int64_t)std::min(num_seqs, kMaxBatch) * num_heads * 8 + 64;
 }
 
 int int4_decode(void *out, const void *q, const int64_t *k_ptrs, const int64_t *v_ptrs, const int64_t *slot_ids,
@@ -755,7 +823,7 @@ int int4_decode(void *out, const void *q, const int64_t *k_ptrs, const int64_t *
   p.max_seq_len = max_seq_len;
   p.out_f32 = out_dtype == VTKV_F32;
   p.scale_log2 = scale * kLog2e;
-  const int j = p.group <= 4 ? 4 : p.group <= 8 ? 2 : 1;
+  const int j = p.group <= 8 ? 2 : 1;
   for (int at = 0; at < num_seqs; at += kMaxBatch) {
     p.num_seqs = std::min(kMaxBatch, num_seqs - at);
     p.q = (const uint16_t *)q + at * q_stride;
@@ -763,17 +831,17 @@ int int4_decode(void *out, const void *q, const int64_t *k_ptrs, const int64_t *
     p.seq_lens = seq_lens + at;
     p.out = (char *)out + (int64_t)at * num_heads * head_size * (p.out_f32 ? 4 : 2);
     size_t lds;
-    const int planned = plan(p, head_size, num_kv_heads, j, lds);
+    const int planned = plan(p, head_size, num_kv_heads, lds);
     if (planned < 0) return planned;
-    const int64_t cum_bytes = ((int64_t)p.num_seqs + 1 + 15) / 16 * 64;
+    const int64_t table = ((int64_t)p.num_seqs * p.chunks * 8 + 63) / 64 * 64;
     const int64_t per_span = 2ll * p.chunk_heads * p.group * (head_size + 2) * 4;
-    const int64_t room = workspace ? (workspace_bytes - cum_bytes) / per_span : 0;
+    const int64_t room = workspace ? (workspace_bytes - table) / per_span : 0;
     if (room < 1 || (uintptr_t)workspace % 16 != 0)
       return fail(VTKV_ENOMEM, "a 16-byte aligned workspace of at least %lld bytes is needed, got %lld",
-                  (long long)(cum_bytes + per_span), (long long)workspace_bytes);
+                  (long long)(table + per_span), (long long)workspace_bytes);
     const int grid = (int)std::min<int64_t>(kDecodeSpans, room);
-    p.cum = (int32_t *)workspace;
-    p.part_o = (float *)((char *)workspace + cum_bytes);
+    p.spans = (int32_t *)workspace;
+    p.part_o = (float *)((char *)workspace + table);
     p.part_ml = p.part_o + 2ll * grid * p.chunk_heads * p.group * head_size;
     const bool f16 = q_dtype == VTKV_F16;
     hipStream_t st = (hipStream_t)stream;

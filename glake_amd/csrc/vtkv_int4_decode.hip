@@ -586,22 +586,27 @@ __global__ void __launch_bounds__(waves_of(D) * 64) int4_decode_kernel(DecodePar
 #pragma unroll 1
       for (int idx = tid; idx < p.chunk_heads * kHeads * kRound * 4; idx += kThreads) {
         const int dq = idx % (kRound * 4), hh = idx / (kRound * 4) % kHeads, at_hs = idx / (kRound * 4) / kHeads;
-        const int v = head_of_chunk(p, c.chunk, at_hs);
+        const int v = p.kv_split == 1 ? c.chunk * p.chunk_heads + at_hs : head_of_chunk(p, c.chunk, at_hs);
         if (dq >= quads || v < 0 || hh >= heads_of(p, v)) continue;
+        // the tiles of the kv head are waves at_hs, at_hs + chunk_heads, ...: two of them at a time
+        const int tiles = p.row_tiles, step = p.chunk_heads;
+        auto wave_of = [&](int t) { return at_hs + min(t, tiles - 1) * step; };
         float m = -INFINITY, l = 0.f, cr = 0.f;
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
-        for (int w = at_hs; w < p.row_tiles * p.chunk_heads; w += p.chunk_heads)
+#pragma unroll 1
+        for (int t = 0; t < tiles; t += 2)
 #pragma unroll
-          for (int jj = 0; jj < J; ++jj) m = fmaxf(m, sml[(w * 16 + jj * kHeads + hh) * 3]);
-        for (int w = at_hs; w < p.row_tiles * p.chunk_heads; w += p.chunk_heads)
+          for (int q = 0; q < 2 * J; ++q) m = fmaxf(m, sml[(wave_of(t + q / J) * 16 + q % J * kHeads + hh) * 3]);
+#pragma unroll 1
+        for (int t = 0; t < tiles; t += 2)
 #pragma unroll
-          for (int jj = 0; jj < J; ++jj) {
-            const int col = jj * kHeads + hh;  // of P; the row of P.V's result
+          for (int q = 0; q < 2 * J; ++q) {
+            const int w = wave_of(t + q / J), col = q % J * kHeads + hh;  // of P; the row of P.V's result
             const float *ml = sml + (w * 16 + col) * 3;
-            const float f = ml[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[0] - m);
-            l += ml[1] * f;
-            cr += ml[2] * f;
+            const float f = ml[0] == -INFINITY || t + q / J >= tiles ? 0.f : __builtin_amdgcn_exp2f(ml[0] - m);
             const float *from = so + (w * kRound + dq / 4) * 256 + (col / 4 * 16 + dq % 4 * 4) * 4 + col % 4;
+            l = __builtin_fmaf(ml[1], f, l);
+            cr = __builtin_fmaf(ml[2], f, cr);
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[i] = __builtin_fmaf(from[4 * i] * 0x1p73f, f, o[i]);  // (133 - 60 binades)
           }
@@ -630,26 +635,30 @@ __global__ void __launch_bounds__(waves_of(D) * 64) int4_decode_kernel(DecodePar
   Cursor lc = cc, now = cc;
   int ahead = 0, first_row = cc.row;  // stages asked for and not yet computed
   bool fresh = true, first_part = true, any = false, aimed = false;
-  auto ask = [&](int next) {  // for two stages from the one that is computed next on
-    for (; ahead < 2 && lc.end > 0; ++ahead) {
+  auto ask = [&](int next, int most) {  // for stages from the one that is computed next on
+    for (; ahead < most && lc.end > 0; ++ahead) {
       if (!aimed) aim(lc);
       issue(lc, next ^ ahead);
       aimed = !step(lc);
     }
   };
   for (int buf = 0;; buf ^= 1) {
-    if (fresh) {  // between two parts (before new loads are asked for: the wait for q would be a wait for them, too)
-      u32x4 raw[kSteps] = {};
-      if (cc.end > 0) load_q(cc, raw);
-      if (any) {
-        finish(now, first_row, first_part, buf ^ 1);
-        if (cc.end == 0) return;
-        first_part = false;
-        first_row = cc.row;
-      }
+    if (fresh && any) {
+      finish(now, first_row, first_part, buf ^ 1);
+      if (cc.end == 0) return;
+      first_part = false;
+      first_row = cc.row;
+    }
+    // a part's first stage is asked for before its q, its second after: the wait for q is a wait for all that was asked
+    // for before
+#pragma unroll 1
+    for (int most = fresh ? 1 : 2;; ++most) {
+      ask(buf, most);
+      if (most == 2) break;
+      u32x4 raw[kSteps];
+      load_q(cc, raw);
       begin(cc, raw);
     }
-    ask(buf);
     wait_loads(ahead == 2 ? 2 * my_loads : 0);
     barrier();
     now = cc;
@@ -659,7 +668,7 @@ __global__ void __launch_bounds__(waves_of(D) * 64) int4_decode_kernel(DecodePar
     barrier();
     --ahead;
     // (the last stage of a part is left to its results)
-    if (!fresh) ask(buf ^ 1);
+    if (!fresh) ask(buf ^ 1, 2);
     compute(now, tile);
     any = true;
   }

@@ -15,7 +15,7 @@ CSRC = os.path.join(_HERE, "csrc")
 LIB_DIR = os.path.join(_HERE, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libvtkv.so")
 SOURCES = ["vtkv_vmm.cpp", "vtkv_cache.hip", "vtkv_attention.hip", "vtkv_attention_f32.hip", "vtkv_prefill.hip",
-           "vtkv_int4_rows.hip", "vtkv_int4_decode.hip", "vtkv_int4_attention.hip", "vtkv_evict.hip"]
+           "vtkv_int4_rows.hip", "vtkv_int4_decode.hip", "vtkv_evict.hip"]
 
 # Packed-FP32 instruction selection is switched off for all device code of this library.
 HIP_FLAGS = [

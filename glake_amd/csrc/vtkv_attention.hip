@@ -1547,14 +1547,14 @@ int attention_impl(void *out, const void *q, const int64_t *k_ptrs, const int64_
                    const void *new_value, int64_t key_stride, int64_t value_stride, const V2Side *v2 = nullptr,
                    bool static_scratch = false) {
   if (kv_dtype == VTKV_INT4) {
-    // 4-bit rows: a kernel of their own (csrc/vtkv_int4_attention.hip); its partial results go behind the counters
+    // 4-bit rows: a kernel of their own (csrc/vtkv_int4_decode.hip); its partial results go behind the counters
     VTKV_REQUIRE(!new_key && !host_seq_lens, "4-bit rows are appended by vtkv_reshape_and_cache");
     VTKV_REQUIRE(!v2, "the split-K interface takes 16-bit, fp8 and float32 caches");
     const int64_t skip = counter_bytes(0, 0);
     const bool usable = workspace && workspace_bytes > skip;
-    return vtkv::int4_attention(out, q, k_ptrs, v_ptrs, slot_ids, seq_lens, nullptr, 0, num_seqs, num_heads,
-                                num_kv_heads, head_size, q_stride, scale, max_seq_len, alibi_slopes, q_dtype, out_dtype,
-                                usable ? (char *)workspace + skip : nullptr, usable ? workspace_bytes - skip : 0, stream);
+    return vtkv::int4_decode(out, q, k_ptrs, v_ptrs, slot_ids, seq_lens, num_seqs, num_heads, num_kv_heads, head_size,
+                             q_stride, scale, max_seq_len, alibi_slopes, q_dtype, out_dtype,
+                             usable ? (char *)workspace + skip : nullptr, usable ? workspace_bytes - skip : 0, stream);
   }
   if (q_dtype == VTKV_F32) {
     // float32 models: a kernel of their own over float32 rows (csrc/vtkv_attention_f32.hip)

@@ -27,15 +27,7 @@ int int4_write_rows(const void *key, const void *value, const int64_t *k_ptrs, c
                     const int64_t *slot_m, const int64_t *slot_ids, const int32_t *seq_lens,
                     const int32_t *cache_seq_lens, int batch, int max_seq_len, int num_heads, int head_size,
                     int64_t key_stride, int64_t value_stride, int src_dtype, void *stream);
-// csrc/vtkv_int4_attention.hip.  units == nullptr: one query row per sequence, seq_lens rows each; otherwise prompt
-// tokens (see vtkv_prefill_attention).
-int int4_attention(void *out, const void *q, const int64_t *k_ptrs, const int64_t *v_ptrs, const int64_t *slot_ids,
-                   const int32_t *seq_lens, const int32_t *units, int unit_tokens, int num_rows, int num_heads,
-                   int num_kv_heads, int head_size, int64_t q_stride, float scale, int max_seq_len,
-                   const float *alibi_slopes, int q_dtype, int out_dtype, void *workspace, int64_t workspace_bytes,
-                   void *stream);
-
-// csrc/vtkv_int4_decode.hip: one query row per sequence; checked arguments (int4_attention)
+// csrc/vtkv_int4_decode.hip
 constexpr int kDecodeSpans = 256;  // workgroups of a launch at most: one per CU
 int64_t int4_decode_workspace_bytes(int num_seqs, int num_heads, int head_size);
 int int4_decode(void *out, const void *q, const int64_t *k_ptrs, const int64_t *v_ptrs, const int64_t *slot_ids,

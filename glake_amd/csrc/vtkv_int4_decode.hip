@@ -817,6 +817,18 @@ int int4_decode(void *out, const void *q, const int64_t *k_ptrs, const int64_t *
                 const int32_t *seq_lens, int num_seqs, int num_heads, int num_kv_heads, int head_size, int64_t q_stride,
                 float scale, int max_seq_len, const float *alibi_slopes, int q_dtype, int out_dtype, void *workspace,
                 int64_t workspace_bytes, void *stream) {
+  VTKV_REQUIRE(out && q && k_ptrs && v_ptrs && slot_ids && seq_lens, "null argument");
+  VTKV_REQUIRE(num_seqs >= 0 && num_heads > 0 && num_kv_heads > 0 && num_heads % num_kv_heads == 0,
+               "num_heads %d must be a positive multiple of num_kv_heads %d", num_heads, num_kv_heads);
+  VTKV_REQUIRE(int4_head_size(head_size), "head_size %d is not supported (64, 80, 96, 112, 128, 256)", head_size);
+  VTKV_REQUIRE(q_dtype == VTKV_BF16 || q_dtype == VTKV_F16, "a 4-bit cache serves bfloat16 and float16 queries");
+  VTKV_REQUIRE(out_dtype == q_dtype || out_dtype == VTKV_F32, "out_dtype must be q_dtype or F32");
+  VTKV_REQUIRE(q_stride >= (int64_t)num_heads * head_size && q_stride % 8 == 0 && (uintptr_t)q % 16 == 0 &&
+                   (uintptr_t)out % 16 == 0,
+               "q and out must be 16-byte aligned, q rows at least num_heads*head_size apart");
+  VTKV_REQUIRE(max_seq_len > 0, "max_seq_len must be > 0");
+  VTKV_REQUIRE(num_heads <= 65535, "too many query heads");
+  VTKV_REQUIRE(int4_row_bytes(num_kv_heads, head_size) < (4 << 20), "rows of 4 MiB and more are not supported");
   const int group_real = num_heads / num_kv_heads, split = vtkv_kv_split(group_real);
   DecodeParams p;
   p.k_ptrs = k_ptrs;

@@ -26,6 +26,12 @@
 //  * fp8 cache: rows are e4m3fn codes (128 bytes per head row); on the way into the LDS stage K is widened
 //    to bf16 and V to fp16 (both exactly), so everything after the stage is the bf16 kernel; the K scale
 //    folds into the logit scale and the V scale into the final normalisation.
+//  * 4-bit cache (vtkv_int4.h): K goes into the stage as bare codes, two masks per pair of them (fp16 denormals c * 2^-24
+//    and c * 2^-20; the queries are brought to fp16 by a power of two per wave, exactly, and carry the rest), so S runs on
+//    the fp16 MFMA for either model type; a row's scale and zero, kept beside the stage, turn its dot products into
+//    logits: x = scale (q . c) + zero sum(q).  V is converted on its way in, c * scale + zero in one rounding to fp16
+//    (2^-12 of the value); scales or zeros beyond the fp16 range take the second pass like large bf16 values, there
+//    rounded to bf16.
 //
 // Otherwise numerics as in the decode kernel (vtkv_attention.hip); the reference computes this with xformers /
 // an external flash-attention kernel (vllm/attention/backends/xformers.py:331-386).
@@ -66,6 +72,7 @@ struct PrefillParams {
   int64_t q_stride;
   int num_heads, num_kv_heads, group;  // (kv heads and heads of each as the kernel sees them: see first_head_of)
   int kv_split, group_real;
+  int row_bytes;     // 4-bit cache: bytes of a row
   float scale_log2;  // scale * log2(e) [* k_scale for an fp8 cache]
   float v_scale;     // 1 for a bf16 cache
 };
@@ -109,14 +116,41 @@ __device__ __forceinline__ u32x4 bf16x8_to_f16x8(u32x4 v) {
     r[i] = pack_f16x2(__builtin_bit_cast(float, v[i] << 16), __builtin_bit_cast(float, v[i] & 0xffff0000u));
   return r;
 }
+// Eight 4-bit codes of a word as fp16 numbers c * 2^-24 (registers 0 and 2) and c * 2^-20 (1 and 3), register r holding
+// codes r and r + 4.
+__device__ __forceinline__ u32x4 codes_to_f16(unsigned w) {
+  const unsigned y = w >> 8;
+  return (u32x4){w & 0x000f000fu, w & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u};
+}
+// The same codes as values code * s + z in order: fp16 (s, z: the row's scale and zero twice in a register each) or bf16.
+__device__ __forceinline__ u32x4 codes_to_values(unsigned w, f16x2 s, f16x2 z) {
+  unsigned v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const f16x2 c = __builtin_bit_cast(f16x2, ((w >> (4 * i)) & 0x000f000fu) | 0x64006400u) - (f16x2){(_Float16)1024.f, (_Float16)1024.f};
+    v[i] = __builtin_bit_cast(unsigned, __builtin_elementwise_fma(c, s, z));
+  }
+  return (u32x4){__builtin_amdgcn_perm(v[1], v[0], 0x05040100u), __builtin_amdgcn_perm(v[3], v[2], 0x05040100u),
+                 __builtin_amdgcn_perm(v[1], v[0], 0x07060302u), __builtin_amdgcn_perm(v[3], v[2], 0x07060302u)};
+}
+__device__ __forceinline__ u32x4 codes_to_bf16(unsigned w, float s, float z) {
+  u32x4 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    r[i] = pack_bf16x2(__builtin_fmaf((float)((w >> (8 * i)) & 15u), s, z), __builtin_fmaf((float)((w >> (8 * i + 4)) & 15u), s, z));
+  return r;
+}
+// KV: what the cache holds, 0 the model's type, 1 e4m3fn codes, 2 4-bit rows.
 // F16: queries, rows and output are fp16 instead of bf16 (rows may still be e4m3fn codes).  S runs on the fp16
 // MFMA and V needs no conversion on its way into LDS; nothing can leave the fp16 range, so there is no second pass.
 // HS: the head size, 64, 80, 96, 112, 128 or 256.  The kernel was shaped for 128, where every constant below has
 // the value it always had.  K rows are held in LDS padded to the MFMA depth of 32 (80 as 96, 112 as 128; the pad
 // is cleared once and q is zero there); V and the output need no padding, every size being a multiple of 16.
 // Above 128 a wave owns one block of 16 columns instead of two.
-template <bool ALIBI, bool FP8, bool F16 = false, int HS = 128>
+template <bool ALIBI, int KV, bool F16 = false, int HS = 128>
 __global__ void __launch_bounds__(kThreads) prefill_attn_kernel(PrefillParams p) {
+  constexpr bool FP8 = KV == 1, I4 = KV == 2;
+  constexpr bool SF16 = F16 || I4;                    // S runs on fp16 operands
   constexpr int kD = HS;                              // (shadows the library-wide 128 inside this kernel)
   constexpr int kHD = (HS + 31) / 32 * 32;            // K row as held in LDS
   constexpr int kRowBytes = kHD * 2 < 256 ? 256 : kHD * 2;  // LDS pitch of a row (16-bit elements)
@@ -146,11 +180,14 @@ __global__ void __launch_bounds__(kThreads) prefill_attn_kernel(PrefillParams p)
   typedef const __attribute__((address_space(1))) char *gptr;
   typedef const __attribute__((address_space(1))) u32x4 *gvec;
   const int64_t slot = p.slot_ids[u_seq];
-  constexpr int kKvRowBytes = FP8 ? kD : 2 * kD;  // bytes of one head row in the cache
+  constexpr int kKvRowBytes = I4 ? kD / 2 : FP8 ? kD : 2 * kD;  // bytes of one head row in the cache (its codes)
   const int kv_real = real_kv_head(p, kvh);  // whose rows this workgroup reads
   gptr k_base = (gptr)(uintptr_t)p.k_ptrs[slot] + kv_real * kKvRowBytes;
   gptr v_base = (gptr)(uintptr_t)p.v_ptrs[slot] + kv_real * kKvRowBytes;
-  const uint32_t row_stride = (uint32_t)(Hkv / p.kv_split) * kKvRowBytes;
+  const uint32_t row_stride = I4 ? (uint32_t)p.row_bytes : (uint32_t)(Hkv / p.kv_split) * kKvRowBytes;
+  // 4-bit rows: from a head's codes to its scale and zero
+  const uint32_t to_pair = (uint32_t)(Hkv / p.kv_split - kv_real) * kKvRowBytes + 4 * kv_real;
+  __shared__ float s_pairs[I4 ? 2 : 1][2][I4 ? kKeyBlock : 1];  // per stage: the K rows' scales, then their zeros
   const int head0 = first_head_of(p, kvh), n_heads = heads_of(p, kvh);
 
   // ---- this wave's columns: block nb, column n -> (token, head); unused columns get q = 0
@@ -175,6 +212,46 @@ __global__ void __launch_bounds__(kThreads) prefill_attn_kernel(PrefillParams p)
       if (kHD == kD || ks * 32 + g * 8 < kD) raw = *reinterpret_cast<const u32x4 *>(qrow + ks * 32 + g * 8);
       if (!valid) raw = (u32x4){0, 0, 0, 0};
       qop[nb][ks] = raw;
+    }
+  }
+  float sl = p.scale_log2;
+  float q_sum[kNB];  // 4-bit rows: sum(q) in the units of the dot products with the codes
+  if constexpr (I4) {
+    float top = 0.f;
+#pragma unroll
+    for (int nb = 0; nb < kNB; ++nb) {
+      q_sum[nb] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < kKS; ++ks)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x = unpack_16<F16>(qop[nb][ks][e >> 1], e & 1);
+          top = fmaxf(top, fabsf(x));
+          q_sum[nb] += x;
+        }
+      q_sum[nb] = sum_over_row_groups(q_sum[nb]);
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+    // the power of two that brings the wave's largest query value near 2^14 in fp16
+    const int expo = min(max((int)(__builtin_bit_cast(unsigned, top) >> 23), 14), 254);
+    const float up = __builtin_bit_cast(float, (unsigned)(268 - expo) << 23);
+    const float per_code = up * 0x1p-24f;  // a dot product with the codes over the one with the values 0..15
+    sl /= per_code;
+#pragma unroll
+    for (int nb = 0; nb < kNB; ++nb) {
+      q_sum[nb] *= per_code;
+#pragma unroll
+      for (int ks = 0; ks < kKS; ++ks) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = unpack_16<F16>(qop[nb][ks][e >> 1], e & 1) * up;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float f = r & 1 ? 0.0625f : 1.f;
+          qop[nb][ks][r] = pack_f16x2(x[r] * f, x[r + 4] * f);
+        }
+      }
     }
   }
   // rows this wave needs: up to the limit of its last used column; its first column's limit says from
@@ -209,7 +286,10 @@ __global__ void __launch_bounds__(kThreads) prefill_attn_kernel(PrefillParams p)
   // stage and is clamped to the same piece of the last row (rows past the end are masked for every column in
   // use, so any finite in-bounds data will do).  Where the pieces do not fill the last load, its idle threads
   // fetch a piece again and store nothing.
-  constexpr int kGp = FP8 ? kD / 16 : kD / 8;
+  // (4-bit rows: pieces of 8 bytes, 16 codes, widened to two pieces like an fp8 one)
+  constexpr int kGp = FP8 || I4 ? kD / 16 : kD / 8;
+  constexpr int kPieceBytes = I4 ? 8 : 16;
+  constexpr bool kPairs = FP8 || I4;
   constexpr int kStagePieces = kKeyBlock * kGp;
   constexpr int kLd = (kStagePieces + kThreads - 1) / kThreads;
   constexpr bool kEvenLd = kStagePieces % kThreads == 0;
@@ -226,19 +306,31 @@ __global__ void __launch_bounds__(kThreads) prefill_attn_kernel(PrefillParams p)
   const uint32_t stage_step = kKeyBlock * row_stride;
   uint32_t ld_off[kLd], last_off[kLd];
 #pragma unroll
-  for (int j = 0; j < kLd; ++j) last_off[j] = (uint32_t)(kv_len - 1) * row_stride + ld_piece[j] * 16;
+  for (int j = 0; j < kLd; ++j) last_off[j] = (uint32_t)(kv_len - 1) * row_stride + ld_piece[j] * kPieceBytes;
   auto rewind = [&]() {
 #pragma unroll
-    for (int j = 0; j < kLd; ++j) ld_off[j] = (uint32_t)ld_row[j] * row_stride + ld_piece[j] * 16;
+    for (int j = 0; j < kLd; ++j) ld_off[j] = (uint32_t)ld_row[j] * row_stride + ld_piece[j] * kPieceBytes;
   };
   rewind();
+  typedef const __attribute__((address_space(1))) u32x2 *gvec2;
+  typedef const __attribute__((address_space(1))) unsigned *gword;
   u32x4 kst[kLd], vst[kLd];
+  unsigned k_pair[kLd], v_pair[kLd];
   auto gload = [&]() {  // loads the next stage's rows and moves on
 #pragma unroll
     for (int j = 0; j < kLd; ++j) {
       const uint32_t off = min(ld_off[j], last_off[j]);
-      kst[j] = *(gvec)(k_base + off);
-      vst[j] = *(gvec)(v_base + off);
+      if constexpr (I4) {
+        const u32x2 k = *(gvec2)(k_base + off), v = *(gvec2)(v_base + off);
+        kst[j] = (u32x4){k[0], k[1], 0, 0};
+        vst[j] = (u32x4){v[0], v[1], 0, 0};
+        const uint32_t pair = off - ld_piece[j] * kPieceBytes + to_pair;
+        k_pair[j] = *(gword)(k_base + pair);
+        v_pair[j] = *(gword)(v_base + pair);
+      } else {
+        kst[j] = *(gvec)(k_base + off);
+        vst[j] = *(gvec)(v_base + off);
+      }
       ld_off[j] += stage_step;
     }
   };
@@ -255,7 +347,7 @@ __global__ void __launch_bounds__(kThreads) prefill_attn_kernel(PrefillParams p)
   int st_k[kLd], st_v[kLd];  // where lstore puts this thread's pieces (fp8: the first of each pair)
 #pragma unroll
   for (int j = 0; j < kLd; ++j) {
-    const int tile = ld_row[j] >> 4, r = ld_row[j] & 15, lp = FP8 ? 2 * ld_piece[j] : ld_piece[j];
+    const int tile = ld_row[j] >> 4, r = ld_row[j] & 15, lp = kPairs ? 2 * ld_piece[j] : ld_piece[j];
     st_k[j] = tile * kTile * kRowBytes + k_lds_offset(r, lp);
     st_v[j] = kKeyBlock * kRowBytes + tile * kTile * kRowBytes + v_lds_offset(r, lp);
   }
@@ -267,7 +359,23 @@ __global__ void __launch_bounds__(kThreads) prefill_attn_kernel(PrefillParams p)
 #pragma unroll
     for (int j = 0; j < kLd; ++j) {
       if (!ld_live[j]) continue;
-      if constexpr (FP8) {
+      if constexpr (I4) {
+        *reinterpret_cast<u32x4 *>(base + st_k[j]) = codes_to_f16(kst[j][0]);
+        *reinterpret_cast<u32x4 *>(base + (st_k[j] ^ 16)) = codes_to_f16(kst[j][1]);
+        const float s = __builtin_bit_cast(float, v_pair[j] << 16), z = __builtin_bit_cast(float, v_pair[j] & 0xffff0000u);
+        if constexpr (WIDE) {
+          *reinterpret_cast<u32x4 *>(base + st_v[j]) = codes_to_bf16(vst[j][0], s, z);
+          *reinterpret_cast<u32x4 *>(base + (st_v[j] ^ 16)) = codes_to_bf16(vst[j][1], s, z);
+        } else {
+          const f16x2 s2 = {(_Float16)s, (_Float16)s}, z2 = {(_Float16)z, (_Float16)z};
+          *reinterpret_cast<u32x4 *>(base + st_v[j]) = codes_to_values(vst[j][0], s2, z2);
+          *reinterpret_cast<u32x4 *>(base + (st_v[j] ^ 16)) = codes_to_values(vst[j][1], s2, z2);
+        }
+        if (ld_piece[j] == 0) {
+          s_pairs[decltype(bufc)::value][0][ld_row[j]] = __builtin_bit_cast(float, k_pair[j] << 16);
+          s_pairs[decltype(bufc)::value][1][ld_row[j]] = __builtin_bit_cast(float, k_pair[j] & 0xffff0000u);
+        }
+      } else if constexpr (FP8) {
         // pieces 2p and 2p+1 of a row sit 16 bytes apart before the swizzle, which flips bit 4 or leaves it
         *reinterpret_cast<u32x4 *>(base + st_k[j]) = fp8x8_widen<F16>(kst[j][0], kst[j][1]);
         *reinterpret_cast<u32x4 *>(base + (st_k[j] ^ 16)) = fp8x8_widen<F16>(kst[j][2], kst[j][3]);
@@ -292,7 +400,6 @@ __global__ void __launch_bounds__(kThreads) prefill_attn_kernel(PrefillParams p)
 #pragma unroll
     for (int db = 0; db < kDB; ++db) vq_off[db] = base + (((2 * db + ((n >> 1) & 1)) ^ swz) << 4);
   }
-  const float sl = p.scale_log2;
   // The reference point of the exponentials only follows the running maximum when that has grown by more
   // than 8 in log2 units (a factor 256 in the weights, harmless in fp32 and fp16): the rescale of the
   // accumulators, which otherwise runs whenever any of the wave's 32 columns sees a new maximum, becomes
@@ -328,8 +435,22 @@ __global__ void __launch_bounds__(kThreads) prefill_attn_kernel(PrefillParams p)
           sacc[nb][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int ks = 0; ks < kKS; ++ks)
-            sacc[nb][t] = mfma_16x16x32<F16>(ka[t][ks], qop[nb][ks], sacc[nb][t]);
+            sacc[nb][t] = mfma_16x16x32<SF16>(ka[t][ks], qop[nb][ks], sacc[nb][t]);
         }
+      if constexpr (I4) {  // dot products with codes to dot products with values (in units of the former)
+        f32x4 ks[2], kz[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          ks[t] = *reinterpret_cast<const f32x4 *>(&s_pairs[buf][0][16 * t + 4 * g]);
+          kz[t] = *reinterpret_cast<const f32x4 *>(&s_pairs[buf][1][16 * t + 4 * g]);
+        }
+#pragma unroll
+        for (int nb = 0; nb < kNB; ++nb)
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sacc[nb][t][r] = __builtin_fmaf(ks[t][r], sacc[nb][t][r], kz[t][r] * q_sum[nb]);
+      }
       // reduction slot (g, j) of the K=32 P.V MFMA stands for row 4g+j of the first tile (j < 4) and row
       // 4g+j-4 of the second (j >= 4), so a lane's A operand is its transposed quad of the first tile
       // followed by that of the second; read once for both column blocks
@@ -450,7 +571,7 @@ __global__ void __launch_bounds__(kThreads) prefill_attn_kernel(PrefillParams p)
 #ifdef VTKV_PREFILL_TRACE
   const unsigned long long trace_t2 = wall_clock64();
 #endif
-  if constexpr (!FP8 && !F16) {
+  if constexpr (!FP8 && (I4 || !F16)) {
     // A V value beyond the fp16 range went into LDS as infinity and has made some accumulator of the workgroup
     // infinite or NaN (a weight of exactly zero gives NaN).  Then the whole unit is computed again with V in
     // bf16; e4m3fn codes always fit fp16.  Inputs that are themselves non-finite take the second pass too and
@@ -549,13 +670,6 @@ int vtkv_prefill_attention(void *out, const void *q, const int64_t *k_ptrs, cons
                "num_heads %d must be a positive multiple of num_kv_heads %d", num_heads, num_kv_heads);
   const int d_index = size_index(head_size);
   VTKV_REQUIRE(d_index >= 0, "head_size %d is not supported (64, 80, 96, 112, 128, 256)", head_size);
-  if (kv_dtype == VTKV_INT4) {
-    const int per_unit = vtkv_prefill_unit_tokens_for(num_heads, num_kv_heads, head_size, kv_dtype);
-    VTKV_REQUIRE(per_unit > 0, "unsupported head counts");
-    return vtkv::int4_attention(out, q, k_ptrs, v_ptrs, slot_ids, nullptr, units, per_unit, num_units * per_unit, num_heads,
-                                num_kv_heads, head_size, q_stride, scale, max_seq_len, alibi_slopes, q_dtype, out_dtype,
-                                nullptr, 0, stream);
-  }
   if (q_dtype == VTKV_F32) {
     // float32 models: every prompt token streams its own rows through the float32 decode kernel
     VTKV_REQUIRE(kv_dtype == VTKV_F32 && out_dtype == VTKV_F32, "float32 queries take a float32 cache and a float32 result");
@@ -569,8 +683,9 @@ int vtkv_prefill_attention(void *out, const void *q, const int64_t *k_ptrs, cons
   VTKV_REQUIRE(q_dtype == VTKV_BF16 || q_dtype == VTKV_F16, "q_dtype must be BF16, F16 or F32");
   VTKV_REQUIRE(out_dtype == q_dtype || out_dtype == VTKV_F32, "out_dtype must be q_dtype or F32");
   VTKV_REQUIRE(scale > 0.f && scale < INFINITY, "scale must be positive and finite");
-  VTKV_REQUIRE(kv_dtype == q_dtype || kv_dtype == VTKV_FP8_E4M3, "kv_dtype must be q_dtype or FP8_E4M3");
-  const bool fp8 = kv_dtype == VTKV_FP8_E4M3;
+  VTKV_REQUIRE(kv_dtype == q_dtype || kv_dtype == VTKV_FP8_E4M3 || kv_dtype == VTKV_INT4,
+               "kv_dtype must be q_dtype, FP8_E4M3 or INT4");
+  const bool fp8 = kv_dtype == VTKV_FP8_E4M3, int4 = kv_dtype == VTKV_INT4;
   if (fp8) VTKV_REQUIRE(k_scale > 0.f && v_scale > 0.f, "fp8 scales must be positive");
   // more than 16 query heads per kv head: several virtual kv heads over the same rows (see first_head_of)
   const int group_real = num_heads / num_kv_heads, split = vtkv_kv_split(group_real);
@@ -579,7 +694,8 @@ int vtkv_prefill_attention(void *out, const void *q, const int64_t *k_ptrs, cons
                    (uintptr_t)out % 16 == 0,
                "q rows must be 16-byte aligned and at least num_heads*head_size apart");
   // (the kernel addresses a sequence's rows with 32-bit byte offsets)
-  VTKV_REQUIRE(max_seq_len > 0 && ((int64_t)max_seq_len + 64) * num_kv_heads * head_size * 2 < (1ll << 31),
+  const int64_t row_bytes = int4 ? vtkv::int4_row_bytes(num_kv_heads, head_size) : (int64_t)num_kv_heads * head_size * 2;
+  VTKV_REQUIRE(max_seq_len > 0 && ((int64_t)max_seq_len + 64) * row_bytes < (1ll << 31),
                "max_seq_len %d: a sequence's K or V range must stay below 2 GiB", max_seq_len);
   VTKV_REQUIRE((int64_t)num_units * kv_virtual < (1ll << 31), "too many units");
   if (num_units == 0) return VTKV_OK;
@@ -598,28 +714,31 @@ int vtkv_prefill_attention(void *out, const void *q, const int64_t *k_ptrs, cons
   p.group = group;
   p.kv_split = split;
   p.group_real = group_real;
+  p.row_bytes = (int)row_bytes;
   p.scale_log2 = scale * kLog2e * (fp8 ? k_scale : 1.f);
   p.v_scale = fp8 ? v_scale : 1.f;
   const dim3 grid((unsigned)((int64_t)num_units * kv_virtual)), block(kThreads);
   hipStream_t st = (hipStream_t)stream;
   // head size 128: one kernel per (type, cache type, ALiBi); the other sizes decide ALiBi at run time
-  static void (*const kKernels[8])(PrefillParams) = {
-      prefill_attn_kernel<false, false, false>, prefill_attn_kernel<true, false, false>,
-      prefill_attn_kernel<false, true, false>,  prefill_attn_kernel<true, true, false>,
-      prefill_attn_kernel<false, false, true>,  prefill_attn_kernel<true, false, true>,
-      prefill_attn_kernel<false, true, true>,   prefill_attn_kernel<true, true, true>,
+  static void (*const kKernels[12])(PrefillParams) = {
+      prefill_attn_kernel<false, 0, false>, prefill_attn_kernel<true, 0, false>, prefill_attn_kernel<false, 1, false>,
+      prefill_attn_kernel<true, 1, false>,  prefill_attn_kernel<false, 2, false>, prefill_attn_kernel<true, 2, false>,
+      prefill_attn_kernel<false, 0, true>,  prefill_attn_kernel<true, 0, true>,  prefill_attn_kernel<false, 1, true>,
+      prefill_attn_kernel<true, 1, true>,   prefill_attn_kernel<false, 2, true>,  prefill_attn_kernel<true, 2, true>,
   };
-#define VTKV_PREFILL_SIZE(HS)                                                                        \
-  prefill_attn_kernel<true, false, false, HS>, prefill_attn_kernel<true, true, false, HS>,           \
-      prefill_attn_kernel<true, false, true, HS>, prefill_attn_kernel<true, true, true, HS>
-  static void (*const kOthers[6][4])(PrefillParams) = {
+#define VTKV_PREFILL_SIZE(HS)                                                                            \
+  prefill_attn_kernel<true, 0, false, HS>, prefill_attn_kernel<true, 1, false, HS>,                      \
+      prefill_attn_kernel<true, 2, false, HS>, prefill_attn_kernel<true, 0, true, HS>,                   \
+      prefill_attn_kernel<true, 1, true, HS>, prefill_attn_kernel<true, 2, true, HS>
+  static void (*const kOthers[6][6])(PrefillParams) = {
       {VTKV_PREFILL_SIZE(64)}, {VTKV_PREFILL_SIZE(80)},  {VTKV_PREFILL_SIZE(96)},
       {VTKV_PREFILL_SIZE(112)}, {VTKV_PREFILL_SIZE(128)}, {VTKV_PREFILL_SIZE(256)},
   };
 #undef VTKV_PREFILL_SIZE
   const bool f16 = q_dtype == VTKV_F16;
-  void (*kernel)(PrefillParams) = head_size == 128 ? kKernels[(f16 ? 4 : 0) + (fp8 ? 2 : 0) + (alibi_slopes ? 1 : 0)]
-                                                   : kOthers[d_index][(f16 ? 2 : 0) + (fp8 ? 1 : 0)];
+  const int kv = int4 ? 2 : fp8 ? 1 : 0;
+  void (*kernel)(PrefillParams) = head_size == 128 ? kKernels[(f16 ? 6 : 0) + 2 * kv + (alibi_slopes ? 1 : 0)]
+                                                   : kOthers[d_index][(f16 ? 3 : 0) + kv];
   hipLaunchKernelGGL(kernel, grid, block, 0, st, p);
   VTKV_HIP(hipGetLastError());
   return VTKV_OK;

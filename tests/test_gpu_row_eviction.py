@@ -234,6 +234,31 @@ def test_evict_lengths_in_place_and_a_loose_bound(env):
     evict_case(env, 16, [5, 0, 3], 50, 10, alias=True)
 
 
+def test_evict_lengths_in_place_for_many_heads(env):
+    """Every kv head of a sequence sees the length as it was, however late it runs."""
+    evict_case(env, 19, [50 + i % 7 for i in range(150)], 50, 10, 16, 64, alias=True)
+
+
+def test_evict_moves_of_many_steps(env):
+    """More moved rows, and more recent ones, than a step of the kernel covers, with and without overlap of the recent rows'
+    old and new places."""
+    evict_case(env, 21, [3000, 2101, 2500], 2100, 2000, 2, 128)
+    evict_case(env, 22, [3000, 2101, 2500], 2100, 700, 2, 112, "int4")
+    evict_case(env, 23, [17000, 16500], 8000, 500, 1, 64)  # (16384 old rows and a few more)
+
+
+def test_evict_negative_nan_stays(env):
+    torch, ops = env
+    w = torch.rand(1, 1, 100, device="cuda")
+    w[0, 0, 17] = torch.tensor([-4194304], dtype=torch.int32).view(torch.float32)[0]  # 0xffc00000
+    w[0, 0, 20] = float("inf")
+    r = S.Ranges(1, 100, 128)
+    r.k[0, :, 0] = torch.arange(100, dtype=torch.uint8, device="cuda")
+    lens = torch.tensor([100], dtype=torch.int32, device="cuda")
+    ops.evict_rows(r.kp, r.vp, w, lens, lens, 11, 10, 100, torch.tensor([0], device="cuda"), 1, 64)
+    assert r.k[0, :11, 0].tolist() == [17] + list(range(90, 100)) and lens.item() == 11
+
+
 def test_evict_many_sequences(env):
     evict_case(env, 17, list(np.random.default_rng(2).integers(0, 60, 700)), 20, 5, 1)
 

@@ -1,9 +1,12 @@
 // Rows of a 4-bit cache written (quantised on the way into each sequence's range) and read back.
 //
 // A head's row takes a team of 16 lanes (32 for head size 256) with eight values each: one 16-byte load, minimum and
-// maximum over the team, one division for the scale, eight codes packed into one 4-byte store.  grid (batch, max_seq_len),
-// one workgroup per token with its K and V heads dealt to the teams.  The bytes of the 16-bit rows bound it (about 4/5
-// of what moves), at decode-step sizes the launch itself.
+// maximum over the team, one division for the scale, eight codes packed into one 4-byte store.  A workgroup takes four
+// tokens, whose K and V heads its teams share out, four loads of a team in flight.
+//   The bytes of the 16-bit rows bound it (about 4/5 of what moves), writing also the 30 instructions per value, at
+// decode-step sizes the launch.  16 000 tokens of 8 kv heads of 128 (67 MB of 16-bit rows, 18 MB of 4-bit ones): written in
+// 27 us, 3.1 TB/s, read back in 21 us, 4.0 TB/s; with one token per workgroup 42 and 32 us, with two 29 and 24, with eight
+// as with four.
 #include "vtkv_common.h"
 #include "vtkv_fp8.h"
 #include "vtkv_int4.h"
@@ -22,16 +25,37 @@ struct RowsParams {
 
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
-// The token of this workgroup: false where there is none; else its row in the cache (per side) and in the tensors.
-__device__ __forceinline__ bool token_of(const RowsParams &p, int64_t &src_row, int64_t &slot, int64_t &off) {
-  const int b = blockIdx.x, t = blockIdx.y;
-  if (p.max_seq_len != 1 && t >= p.seq_lens[b]) return false;
-  off = p.slot_m[b];
-  if (off < 0) return false;
-  off += (int64_t)t * p.row_bytes;
-  slot = p.slot_ids[b];
-  src_row = p.max_seq_len == 1 ? (int64_t)b : (int64_t)p.cache_seq_lens[b] + t;
-  return true;
+constexpr int kTokens = 4;  // of a workgroup, one behind the other
+constexpr int kAhead = 4;   // head rows that a team asks for before it works on the first
+
+// The tokens of this workgroup: how many, the first one's row in the tensors, and where its cache rows are.
+struct Tokens {
+  int rows;
+  int64_t first;
+  char *k, *v;
+};
+__device__ __forceinline__ Tokens tokens_of(const RowsParams &p) {
+  const int b = blockIdx.x, t0 = blockIdx.y * kTokens;
+  Tokens t;
+  t.rows = p.max_seq_len == 1 ? 1 : min(kTokens, min(p.seq_lens[b], p.max_seq_len) - t0);
+  const int64_t off = p.slot_m[b];
+  if (off < 0) t.rows = 0;
+  if (t.rows <= 0) return t;
+  const int64_t slot = p.slot_ids[b], at = off + (int64_t)t0 * p.row_bytes;
+  t.k = reinterpret_cast<char *>(p.k_ptrs[slot]) + at;
+  t.v = reinterpret_cast<char *>(p.v_ptrs[slot]) + at;
+  t.first = p.max_seq_len == 1 ? (int64_t)b : (int64_t)p.cache_seq_lens[b] + t0;
+  return t;
+}
+
+// Item i of a workgroup: (token, K or V, head).
+struct Item {
+  int token, head;
+  bool is_v;
+};
+__device__ __forceinline__ Item item_of(int i, int num_heads) {
+  const int token = (int)((unsigned)i / (unsigned)(2 * num_heads)), hr = i - token * 2 * num_heads;
+  return {token, hr >= num_heads ? hr - num_heads : hr, hr >= num_heads};
 }
 
 template <bool F16>
@@ -41,98 +65,140 @@ __device__ __forceinline__ float widen(unsigned pair, int which) {
   return vtkv::bf16_bits_to_f32(h);
 }
 
+// A value joined over each team's lanes, neighbours first.
+template <int TEAM, typename Op>
+__device__ __forceinline__ float over_team(float x, Op op) {
+#define VTKV_JOIN(CTRL) \
+  x = op(x, vtkv::bits_f32((unsigned)__builtin_amdgcn_update_dpp(0, (int)vtkv::f32_bits(x), CTRL, 0xf, 0xf, true)))
+  VTKV_JOIN(0xb1);   // lanes 1 0 3 2 of each four
+  VTKV_JOIN(0x4e);   // 2 3 0 1
+  VTKV_JOIN(0x141);  // each eight mirrored
+  VTKV_JOIN(0x140);  // each sixteen mirrored
+#undef VTKV_JOIN
+  if constexpr (TEAM == 32) x = op(x, __shfl_xor(x, 16, 32));
+  return x;
+}
+
 template <bool F16, bool ALIGNED, int TEAM>
 __global__ void __launch_bounds__(kThreads) int4_write_kernel(RowsParams p) {
-  int64_t src_row, slot, off;
-  if (!token_of(p, src_row, slot, off)) return;
+  const Tokens t = tokens_of(p);
   const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
-  const int half = p.head_size / 2;
+  const int half = p.head_size / 2, items = max(t.rows, 0) * 2 * p.num_heads;
   const bool live = 8 * lane < p.head_size;
-  for (int hr = team; hr < 2 * p.num_heads; hr += kThreads / TEAM) {
-    const bool is_v = hr >= p.num_heads;
-    const int head = is_v ? hr - p.num_heads : hr;
-    const char *src = (is_v ? p.value + src_row * p.value_stride * 2 : p.key + src_row * p.key_stride * 2) +
-                      ((int64_t)head * p.head_size + 8 * lane) * 2;
-    char *row = reinterpret_cast<char *>(is_v ? p.v_ptrs[slot] : p.k_ptrs[slot]) + off;
-    u32x4 raw = {0, 0, 0, 0};
-    if (live) {
+  constexpr int kTeams = kThreads / TEAM;
+  for (int i0 = team; i0 < items; i0 += kTeams * kAhead) {
+    u32x4 raws[kAhead];
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+      const Item it = item_of(min(i0 + a * kTeams, items - 1), p.num_heads);  // (past the end: the last one, not written)
+      const int64_t src_row = t.first + it.token;
+      const char *src = (it.is_v ? p.value + src_row * p.value_stride * 2 : p.key + src_row * p.key_stride * 2) +
+                        ((int64_t)it.head * p.head_size + 8 * (live ? lane : 0)) * 2;
       if constexpr (ALIGNED) {
-        raw = *reinterpret_cast<const u32x4 *>(src);
+        raws[a] = *reinterpret_cast<const u32x4 *>(src);
       } else {
         const uint16_t *e = reinterpret_cast<const uint16_t *>(src);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) raw[i] = (unsigned)e[2 * i] | (unsigned)e[2 * i + 1] << 16;
+        for (int i = 0; i < 4; ++i) raws[a][i] = (unsigned)e[2 * i] | (unsigned)e[2 * i + 1] << 16;
       }
     }
-    float x[8], lo = INFINITY, hi = -INFINITY;
-    bool odd = false;  // a value that is not finite
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      x[i] = widen<F16>(raw[i >> 1], i & 1);
-      odd |= (vtkv::f32_bits(x[i]) & 0x7f800000u) == 0x7f800000u;
-      lo = fminf(lo, x[i]);
-      hi = fmaxf(hi, x[i]);
-    }
-    if (!live) lo = INFINITY, hi = -INFINITY;
+    for (int a = 0; a < kAhead; ++a) {
+      if (i0 + a * kTeams >= items) break;
+      const Item it = item_of(i0 + a * kTeams, p.num_heads);
+      const int head = it.head;
+      char *row = (it.is_v ? t.v : t.k) + (int64_t)it.token * p.row_bytes;
+      const u32x4 raw = live ? raws[a] : (u32x4){0, 0, 0, 0};
+      float x[8], lo = INFINITY, hi = -INFINITY, finite = 0.f;
 #pragma unroll
-    for (int d = 1; d < TEAM; d <<= 1) {
-      lo = fminf(lo, __shfl_xor(lo, d, TEAM));
-      hi = fmaxf(hi, __shfl_xor(hi, d, TEAM));
-    }
-    const unsigned long long any = __ballot(odd);
-    const unsigned long long mine = (any >> ((threadIdx.x & 63) / TEAM * TEAM)) & ((1ull << TEAM) - 1);
-    unsigned zero16 = vtkv::f32_to_bf16_bits_rne(lo);
-    const float zero = vtkv::bf16_bits_to_f32((uint16_t)zero16);
-    const float range = hi - zero;
-    unsigned scale16 = vtkv::f32_to_bf16_bits_rne(range / 15.0f);
-    float scale = vtkv::bf16_bits_to_f32((uint16_t)scale16);
-    if (scale < 1.17549435e-38f) scale = 0.f, scale16 = 0;  // (also a negative one: every value equal, zero rounded up)
-    const bool bad = mine != 0 || (vtkv::f32_bits(range) & 0x7f800000u) == 0x7f800000u;
-    const float inverse = scale > 0.f ? __builtin_amdgcn_rcpf(scale) : 0.f;
-    unsigned word = 0;
+      for (int i = 0; i < 8; ++i) {
+        x[i] = widen<F16>(raw[i >> 1], i & 1);
+        finite = __builtin_fmaf(x[i], 0.f, finite);  // (NaN from the first infinity or NaN on)
+        lo = fminf(lo, x[i]);
+        hi = fmaxf(hi, x[i]);
+      }
+      if (!live) lo = INFINITY, hi = -INFINITY;
+      lo = over_team<TEAM>(lo, [](float u, float v) { return fminf(u, v); });
+      hi = over_team<TEAM>(hi, [](float u, float v) { return fmaxf(u, v); });
+      const unsigned long long any = __ballot(finite != 0.f);
+      const unsigned long long mine = (any >> ((threadIdx.x & 63) / TEAM * TEAM)) & ((1ull << TEAM) - 1);
+      unsigned zero16 = vtkv::f32_to_bf16_bits_rne(lo);
+      const float zero = vtkv::bf16_bits_to_f32((uint16_t)zero16);
+      const float range = hi - zero;
+      unsigned scale16 = vtkv::f32_to_bf16_bits_rne(range / 15.0f);
+      float scale = vtkv::bf16_bits_to_f32((uint16_t)scale16);
+      const bool bad = mine != 0 || (vtkv::f32_bits(range) & 0x7f800000u) == 0x7f800000u;
+      float half_step = 0.5f * scale, inverse = __builtin_amdgcn_rcpf(scale) * (1.f - 0x1p-20f);
+      if (bad || scale < 1.17549435e-38f)  // (a negative one, too: every value equal, zero rounded up)
+        scale = inverse = 0.f, scale16 = 0, half_step = INFINITY;
+      unsigned word = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      // The quotient's nearest code first, then the exact remainder against half a step: a value on the border
-      // between two codes takes the upper one, whatever the reciprocal's last bit is.  (16-bit values over a bf16
-      // step meet that border in one of some hundred values.)
-      const float d = x[i] - zero;
-      float c = __builtin_rintf(d * inverse);
-      const float rest = 2.f * __builtin_fmaf(-c, scale, d);
-      c += rest >= scale ? 1.f : rest < -scale ? -1.f : 0.f;
-      const int code = scale > 0.f && !bad ? (int)fminf(fmaxf(c, 0.f), 15.f) : 0;
-      word |= (unsigned)code << (4 * i);
+      for (int i = 0; i < 8; ++i) {
+        // The quotient's code or the one below it (the reciprocal is cut by more than it can be too large), then the exact
+        // remainder against half a step: a value on the border between two codes takes the upper one.  (16-bit values over a
+        // bf16 step meet that border in one of some hundred values.)
+        const float d = x[i] - zero, c = __builtin_floorf(__builtin_fmaf(d, inverse, 0.5f));
+        const int code = (int)c + (__builtin_fmaf(-c, scale, d) >= half_step ? 1 : 0);
+        word |= (unsigned)min(max(code, 0), 15) << (4 * i);
+      }
+      if (bad) scale16 = zero16 = 0x7fc0u;
+      if (live) *reinterpret_cast<unsigned *>(row + head * half + 4 * lane) = word;
+      if (lane == 0) *reinterpret_cast<unsigned *>(row + p.num_heads * half + 4 * head) = scale16 | zero16 << 16;
+      if (head == p.num_heads - 1)
+        for (int i = p.num_heads * (half + 4) + 4 * lane; i < p.row_bytes; i += 4 * TEAM)
+          *reinterpret_cast<unsigned *>(row + i) = 0;
     }
-    if (bad) scale16 = zero16 = 0x7fc0u;
-    if (live) *reinterpret_cast<unsigned *>(row + head * half + 4 * lane) = word;
-    if (lane == 0) *reinterpret_cast<unsigned *>(row + p.num_heads * half + 4 * head) = scale16 | zero16 << 16;
-    if (head == p.num_heads - 1)
-      for (int i = p.num_heads * (half + 4) + 4 * lane; i < p.row_bytes; i += 4 * TEAM)
-        *reinterpret_cast<unsigned *>(row + i) = 0;
   }
 }
 
-template <int DT>
+template <int DT, bool ALIGNED, int TEAM>
 __global__ void __launch_bounds__(kThreads) int4_read_kernel(RowsParams p) {
-  int64_t dst_row, slot, off;
-  if (!token_of(p, dst_row, slot, off)) return;
-  const int half = p.head_size / 2, words = p.head_size / 8;  // (a word: eight codes)
-  for (int i = threadIdx.x; i < 2 * p.num_heads * words; i += kThreads) {
-    const bool is_v = i >= p.num_heads * words;
-    const int j = is_v ? i - p.num_heads * words : i;
-    const int head = j / words, at = j % words;
-    const char *row = reinterpret_cast<const char *>(is_v ? p.v_ptrs[slot] : p.k_ptrs[slot]) + off;
-    const unsigned codes = *reinterpret_cast<const unsigned *>(row + head * half + 4 * at);
-    const unsigned sz = *reinterpret_cast<const unsigned *>(row + p.num_heads * half + 4 * head);
-    const float scale = vtkv::bits_f32(sz << 16), zero = vtkv::bits_f32(sz & 0xffff0000u);
-    char *dst = const_cast<char *>(is_v ? p.value : p.key);
-    const int64_t e0 = dst_row * (is_v ? p.value_stride : p.key_stride) + (int64_t)head * p.head_size + 8 * at;
+  const Tokens t = tokens_of(p);
+  const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
+  const int half = p.head_size / 2, items = max(t.rows, 0) * 2 * p.num_heads;
+  if (8 * lane >= p.head_size) return;
+  constexpr int kTeams = kThreads / TEAM;
+  for (int i0 = team; i0 < items; i0 += kTeams * kAhead) {
+    unsigned codes[kAhead], pairs[kAhead];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      // (code * scale has 12 significant bits: the one rounding to fp32 is the addition's)
-      const float x = __builtin_fmaf((float)((codes >> (4 * e)) & 15u), scale, zero);
-      if constexpr (DT == VTKV_F32) reinterpret_cast<float *>(dst)[e0 + e] = x;
-      else if constexpr (DT == VTKV_BF16) reinterpret_cast<uint16_t *>(dst)[e0 + e] = vtkv::f32_to_bf16_bits_rne(x);
-      else reinterpret_cast<_Float16 *>(dst)[e0 + e] = (_Float16)x;
+    for (int a = 0; a < kAhead; ++a) {
+      const Item it = item_of(min(i0 + a * kTeams, items - 1), p.num_heads);
+      const char *row = (it.is_v ? t.v : t.k) + (int64_t)it.token * p.row_bytes;
+      codes[a] = *reinterpret_cast<const unsigned *>(row + it.head * half + 4 * lane);
+      pairs[a] = *reinterpret_cast<const unsigned *>(row + p.num_heads * half + 4 * it.head);
+    }
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+      if (i0 + a * kTeams >= items) break;
+      const Item it = item_of(i0 + a * kTeams, p.num_heads);
+      const float scale = vtkv::bits_f32(pairs[a] << 16), zero = vtkv::bits_f32(pairs[a] & 0xffff0000u);
+      char *dst = const_cast<char *>(it.is_v ? p.value : p.key);
+      const int64_t e0 = (t.first + it.token) * (it.is_v ? p.value_stride : p.key_stride) + (int64_t)it.head * p.head_size + 8 * lane;
+      constexpr int kElem = DT == VTKV_F32 ? 4 : 2;
+      unsigned out[2 * kElem];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        // (code * scale has 12 significant bits: the one rounding to fp32 is the addition's)
+        const float x = __builtin_fmaf((float)((codes[a] >> (4 * e)) & 15u), scale, zero);
+        if constexpr (DT == VTKV_F32) {
+          out[e] = vtkv::f32_bits(x);
+        } else {
+          const unsigned h = DT == VTKV_BF16 ? (unsigned)vtkv::f32_to_bf16_bits_rne(x)
+                                             : (unsigned)__builtin_bit_cast(unsigned short, (_Float16)x);
+          out[e / 2] = e & 1 ? out[e / 2] | h << 16 : h;
+        }
+      }
+      if constexpr (ALIGNED) {
+#pragma unroll
+        for (int w = 0; w < 2 * kElem; w += 4)
+          *reinterpret_cast<u32x4 *>(dst + e0 * kElem + 4 * w) = (u32x4){out[w], out[w + 1], out[w + 2], out[w + 3]};
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if constexpr (DT == VTKV_F32) reinterpret_cast<unsigned *>(dst)[e0 + e] = out[e];
+          else reinterpret_cast<uint16_t *>(dst)[e0 + e] = (uint16_t)(out[e / 2] >> (16 * (e & 1)));
+        }
+      }
     }
   }
 }
@@ -168,7 +234,7 @@ int int4_write_rows(const void *key, const void *value, const int64_t *k_ptrs, c
                         max_seq_len, num_heads, head_size, (int)int4_row_bytes(num_heads, head_size), key_stride,
                         value_stride};
   const bool aligned = key_stride % 8 == 0 && value_stride % 8 == 0 && (uintptr_t)key % 16 == 0 && (uintptr_t)value % 16 == 0;
-  const dim3 grid((unsigned)batch, (unsigned)max_seq_len);
+  const dim3 grid((unsigned)batch, (unsigned)((max_seq_len + kTokens - 1) / kTokens));
   hipStream_t st = (hipStream_t)stream;
 #define VTKV_INT4_WRITE(F, A)                                                                        \
   do {                                                                                               \
@@ -210,11 +276,20 @@ int vtkv_read_cached_rows(void *key, void *value, const int64_t *k_ptrs, const i
   const RowsParams p = {(const char *)key, (const char *)value, k_ptrs, v_ptrs, slot_m, slot_ids, seq_lens, cache_seq_lens,
                         max_seq_len, num_heads, head_size, (int)vtkv::int4_row_bytes(num_heads, head_size), key_stride,
                         value_stride};
-  const dim3 grid((unsigned)batch, (unsigned)max_seq_len);
+  const dim3 grid((unsigned)batch, (unsigned)((max_seq_len + kTokens - 1) / kTokens));
   hipStream_t st = (hipStream_t)stream;
-  if (dst_dtype == VTKV_F32) hipLaunchKernelGGL(int4_read_kernel<VTKV_F32>, grid, dim3(kThreads), 0, st, p);
-  else if (dst_dtype == VTKV_BF16) hipLaunchKernelGGL(int4_read_kernel<VTKV_BF16>, grid, dim3(kThreads), 0, st, p);
-  else hipLaunchKernelGGL(int4_read_kernel<VTKV_F16>, grid, dim3(kThreads), 0, st, p);
+  const int esize = dst_dtype == VTKV_F32 ? 4 : 2;
+  const bool aligned = key_stride * esize % 16 == 0 && value_stride * esize % 16 == 0 && (uintptr_t)key % 16 == 0 && (uintptr_t)value % 16 == 0;
+  typedef void (*Kernel)(RowsParams);
+  static const Kernel kernels[3][2][2] = {
+      {{int4_read_kernel<VTKV_F32, false, 16>, int4_read_kernel<VTKV_F32, false, 32>},
+       {int4_read_kernel<VTKV_F32, true, 16>, int4_read_kernel<VTKV_F32, true, 32>}},
+      {{int4_read_kernel<VTKV_BF16, false, 16>, int4_read_kernel<VTKV_BF16, false, 32>},
+       {int4_read_kernel<VTKV_BF16, true, 16>, int4_read_kernel<VTKV_BF16, true, 32>}},
+      {{int4_read_kernel<VTKV_F16, false, 16>, int4_read_kernel<VTKV_F16, false, 32>},
+       {int4_read_kernel<VTKV_F16, true, 16>, int4_read_kernel<VTKV_F16, true, 32>}}};
+  const int type = dst_dtype == VTKV_F32 ? 0 : dst_dtype == VTKV_BF16 ? 1 : 2;
+  hipLaunchKernelGGL(kernels[type][aligned][head_size > 128], grid, dim3(kThreads), 0, st, p);
   VTKV_HIP(hipGetLastError());
   return VTKV_OK;
 }

@@ -27,8 +27,16 @@
 // and the two 16-row tiles of a wave share one tile of logits (J = 2), so the softmax arithmetic is per logit that
 // exists; P.V takes the same layout with zeros where a row is not the part's, and the parts are added up at the end.
 //
-// The batch's rows in steps of 16 are cut into as many equal spans as workgroups run; a span that ends inside a
-// sequence leaves a partial result in the workspace and a second kernel merges them.
+// The batch's rows in steps of 16 are cut into as many equal spans as workgroups run, where a sequence that begins counts
+// as some steps more (part_units): a new part costs as much time as three stages, and without that count the workgroup
+// with the most parts ends last (17 sequences of 3 to 2501 rows, 32 kv heads of 80 in four chunks: 53 us against 32 us when
+// the end of a part took 4.5 us; two stages 35 us, four 32 us).  A span that ends inside a sequence leaves a partial
+// result in the workspace and a second kernel merges them.
+//
+// What it takes (kernel and merge): 64 sequences of 512 to 4096 rows of 8 kv heads of 128, 4 query heads each (161 MB): 43 + 5
+// us; four of 32768 to 131072 rows (371 MB): 77 + 5 us; 32 kv heads of 80 as above (60 MB): 30 + 4 us; one of 777 rows: 16 + 4
+// us.  A stage takes 2.85 us with all workgroups at it (6.3 TB/s), the way to the first stage's rows 8.5 us, the end of a
+// part 2.5 to 4 us.
 #include "vtkv_attn_common.h"
 #include "vtkv_common.h"
 #include "vtkv_int4.h"
@@ -49,8 +57,9 @@ constexpr int kLdsBytes = 160 * 1024;
 
 constexpr int waves_of(int d) { return d > 128 ? 8 : 16; }
 constexpr int loads_of(int d) { return d > 128 ? 5 : 3; }  // 16-byte loads per lane, stage and side at most
-// blocks of 16 columns that all waves' results go through LDS at a time (what a stage of whole rows holds)
-constexpr int round_of(int d) { return d > 128 ? 8 : d / 32; }
+// blocks of 16 columns of 16 rows that all waves' results go through LDS at a time: half of them (all, where two parts of a
+// column are added up before)
+constexpr int round_of(int d) { return (d / 16 + 1) / 2; }
 constexpr int results_bytes(int d) { return waves_of(d) * (round_of(d) * 1024 + 192); }
 
 struct DecodeParams {
@@ -70,10 +79,12 @@ struct DecodeParams {
   int stage_bytes;             // LDS of a stage: K, then V (or what its waves hold, combined when a part ends)
   int code_units, scale_units; // 16-byte pieces of a row in LDS
   int min_units;               // a span's units at least
+  int part_units;              // what beginning a sequence counts
   float scale_log2;
 };
 
-// The spans: unit u of the batch belongs to span u * active / total, each a contiguous range.
+// The spans: the batch's units are numbered through, part_units of each sequence (per chunk) that stand for no rows and
+// then its rows' units; unit u belongs to span u * active / total, each a contiguous range.
 __device__ __forceinline__ int active_spans(const DecodeParams &p, int total, int grid) {
   return max(1, min(grid, total / p.min_units));
 }
@@ -163,7 +174,10 @@ __global__ void __launch_bounds__(waves_of(D) * 64) int4_decode_kernel(DecodePar
     for (int k = 0; k < kPer; ++k) {
       const int idx = tid * kPer + k;
       local[k] = sum;
-      if (idx < B) sum += (max(0, min(p.seq_lens[idx], p.max_seq_len)) + kUnitRows - 1) / kUnitRows;
+      if (idx < B) {
+        const int rows = min(p.seq_lens[idx], p.max_seq_len);
+        if (rows > 0) sum += (rows - 1) / kUnitRows + 1 + p.part_units;
+      }
     }
     if (in_table) {
       s_ptr[2 * tid] = (uint64_t)p.k_ptrs[slot];
@@ -200,14 +214,15 @@ __global__ void __launch_bounds__(waves_of(D) * 64) int4_decode_kernel(DecodePar
     const DecodeParams &p = reload();
     return uniform(min(p.seq_lens[b], p.max_seq_len));
   };
-  // the part of sequence b, chunk c from unit k on, as far as `left` units go
+  // the part of sequence b, chunk c from unit k on, as far as `left` units go (none, if they end before its rows begin)
+  const int part_units = p.part_units;
   auto enter = [&](Cursor &c, int b, int chunk, int k, int left) {
     const int nb = uniform(s_cum[b + 1]) - uniform(s_cum[b]);
     const int take = min(left, nb - k);
     c.b = b;
     c.chunk = chunk;
-    c.row = k * kUnitRows;
-    c.end = min(len_of(b), (k + take) * kUnitRows);
+    c.row = max(0, k - part_units) * kUnitRows;
+    c.end = min(len_of(b), max(0, k + take - part_units) * kUnitRows);
     c.left = left - take;
   };
   auto step = [&](Cursor &c) {  // one stage on; true: into another part
@@ -239,6 +254,7 @@ __global__ void __launch_bounds__(waves_of(D) * 64) int4_decode_kernel(DecodePar
     const int c0 = uniform(s_cum[b]), nb = uniform(s_cum[b + 1]) - c0;
     const int k = u_begin - c0 * C;
     enter(cc, b, k / nb, k % nb, u_end - u_begin);
+    if (cc.end == 0) return;
   }
 
   // ---- this wave's kv head and rows of the stage
@@ -264,8 +280,8 @@ __global__ void __launch_bounds__(waves_of(D) * 64) int4_decode_kernel(DecodePar
   // piece (wave + waves * k) * 64 + l
   const int pieces = stage_rows * units_row, num_loads = (pieces + 63) / 64;
   const int my_loads = wave < num_loads ? (num_loads - wave + kWaves - 1) / kWaves : 0;
-  int ld_row[kLoads];   // its row of the stage, and where its piece begins in a row of the cursor's chunk
-  int ld_at[kLoads];
+  // its row of the stage (10 bits) and where its piece begins in a row of the cursor's chunk (22: a row is below 4 MiB)
+  unsigned ld_at[kLoads];
   uint64_t k_from, v_from;  // the cursor's first row
   auto aim = [&](const Cursor &c) {  // at the cursor's part
     const DecodeParams &p = reload();
@@ -276,9 +292,8 @@ __global__ void __launch_bounds__(waves_of(D) * 64) int4_decode_kernel(DecodePar
 #pragma unroll
     for (int k = 0; k < kLoads; ++k) {
       const int i = (wave + kWaves * k) * 64 + opaque(lane);
-      ld_row[k] = i / units_row;
-      const int col = i - ld_row[k] * units_row;
-      ld_at[k] = col * 16 + (col < p.code_units ? code0 : scale0);
+      const int row = i / units_row, col = i - row * units_row;
+      ld_at[k] = (unsigned)row << 22 | (unsigned)(col * 16 + (col < p.code_units ? code0 : scale0));
     }
     uint64_t kb, vb;
     if (c.b < kPtrTable) {
@@ -300,7 +315,7 @@ __global__ void __launch_bounds__(waves_of(D) * 64) int4_decode_kernel(DecodePar
 #pragma unroll
     for (int k = 0; k < kLoads; ++k) {
       if (wave + kWaves * k >= num_loads) break;
-      const uint32_t off = __umul24(min(ld_row[k], last), p.row_bytes) + ld_at[k];  // (a row is below 4 MiB)
+      const uint32_t off = __umul24(min((int)(ld_at[k] >> 22), last), p.row_bytes) + (ld_at[k] & 0x3fffffu);
       if ((wave + kWaves * k) * 64 + lane < pieces) {
         load_to_lds(k_from, off, dst + k * kWaves * 1024);
         load_to_lds(v_from, off, dst + k * kWaves * 1024 + side_bytes);
@@ -554,11 +569,13 @@ __global__ void __launch_bounds__(waves_of(D) * 64) int4_decode_kernel(DecodePar
     }
   };
 
-  // ---- the end of a part: what the waves of a kv head hold (row tiles, and the parts of a column) is added up through
-  // the stage that has been used up, some blocks of columns at a time, and stored: the result, or this span's share of one
+  // ---- the end of a part: the waves of a kv head (row tiles, and the parts of a column) first agree on the maximum, bring
+  // their sums to it and add up the parts in registers, then the tiles through the stage that has been used up: each of
+  // the head's waves adds up some blocks of columns and stores them: the result, or this span's share of one
   auto finish = [&](const Cursor &c, int first_row, bool first_part, int buf) {
     const DecodeParams &p = reload();
     const int tid = opaque(threadIdx.x), lane = tid & 63, g = lane >> 4, n = lane & 15;
+    constexpr int kVals = J == 2 ? 2 : 4, kPer = kRound * J;  // rows of a block per lane; blocks of columns of a round
     l_run = sum_over_row_groups(l_run);
     z_run = sum_over_row_groups(z_run);
     float *so = reinterpret_cast<float *>(smem + buf * p.stage_bytes), *sml = so + kWaves * kRound * 256;
@@ -574,61 +591,84 @@ __global__ void __launch_bounds__(waves_of(D) * 64) int4_decode_kernel(DecodePar
       if (first_row == 0) span[0] = place;
       if (c.end == len) span[1] = blockIdx.x;
     }
+    barrier();
+    // the tiles of the kv head are waves hs, hs + chunk_heads, ...; this lane: query head n % kHeads
+    const int tiles = p.row_tiles, tile_step = p.chunk_heads;
+    float m = -INFINITY, l = 0.f, cr = 0.f;
+    const float *ml0 = sml + (hs * 16 + n % kHeads) * 3;
 #pragma unroll 1
-    for (int d0 = 0; d0 < kDB; d0 += kRound) {
+    for (int t = 0; t < tiles; ++t)
 #pragma unroll
-      for (int d = 0; d < kDB; ++d)
-        if (d / kRound * kRound == d0)
-          *reinterpret_cast<f32x4 *>(so + (wave * kRound + d % kRound) * 256 + lane * 4) = acc[d];
-      barrier();
-      // one thread: four neighbouring columns of one query head
-      const int quads = min(kRound, kDB - d0) * 4;
+      for (int q = 0; q < J; ++q) m = fmaxf(m, ml0[(t * tile_step * 16 + q * kHeads) * 3]);
 #pragma unroll 1
-      for (int idx = tid; idx < p.chunk_heads * kHeads * kRound * 4; idx += kThreads) {
-        const int dq = idx % (kRound * 4), hh = idx / (kRound * 4) % kHeads, at_hs = idx / (kRound * 4) / kHeads;
-        const int v = p.kv_split == 1 ? c.chunk * p.chunk_heads + at_hs : head_of_chunk(p, c.chunk, at_hs);
-        if (dq >= quads || v < 0 || hh >= heads_of(p, v)) continue;
-        // the tiles of the kv head are waves at_hs, at_hs + chunk_heads, ...: two of them at a time
-        const int tiles = p.row_tiles, step = p.chunk_heads;
-        auto wave_of = [&](int t) { return at_hs + min(t, tiles - 1) * step; };
-        float m = -INFINITY, l = 0.f, cr = 0.f;
-        f32x4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-        for (int t = 0; t < tiles; t += 2)
+    for (int t = 0; t < tiles; ++t)
 #pragma unroll
-          for (int q = 0; q < 2 * J; ++q) m = fmaxf(m, sml[(wave_of(t + q / J) * 16 + q % J * kHeads + hh) * 3]);
-#pragma unroll 1
-        for (int t = 0; t < tiles; t += 2)
+      for (int q = 0; q < J; ++q) {
+        const float *ml = ml0 + (t * tile_step * 16 + q * kHeads) * 3;
+        const float f = ml[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[0] - m);
+        l = __builtin_fmaf(ml[1], f, l);
+        cr = __builtin_fmaf(ml[2], f, cr);
+      }
+    rescale(lazy == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_ref - m) * 0x1p73f);  // (133 - 60 binades)
+    const int hv = head < 0 ? 0 : heads_of(p, head);
+    const int64_t part = ((int64_t)place * p.chunk_heads + hs) * p.group;
+    if (!whole && rt == 0 && lane < hv)  // (hv <= kHeads)
+      *reinterpret_cast<u32x2 *>(p.part_ml + (part + lane) * 2) = (u32x2){__builtin_bit_cast(unsigned, m), __builtin_bit_cast(unsigned, l)};
+    // the rows (query heads) that this lane holds of a block, and what they take
+    auto row_of = [&](int k) { return J == 2 ? 4 * (g & 1) + 2 * k + (lane >> 5) : 4 * g + k; };
+    const float factor = whole ? 1.f / l : 1.f;
+    float add[kVals], mul[kVals];
 #pragma unroll
-          for (int q = 0; q < 2 * J; ++q) {
-            const int w = wave_of(t + q / J), col = q % J * kHeads + hh;  // of P; the row of P.V's result
-            const float *ml = sml + (w * 16 + col) * 3;
-            const float f = ml[0] == -INFINITY || t + q / J >= tiles ? 0.f : __builtin_amdgcn_exp2f(ml[0] - m);
-            const float *from = so + (w * kRound + dq / 4) * 256 + (col / 4 * 16 + dq % 4 * 4) * 4 + col % 4;
-            l = __builtin_fmaf(ml[1], f, l);
-            cr = __builtin_fmaf(ml[2], f, cr);
+    for (int k = 0; k < kVals; ++k) {
+      add[k] = __shfl(cr, row_of(k));
+      mul[k] = __shfl(factor, row_of(k));
+    }
+    typedef float Vals __attribute__((ext_vector_type(kVals)));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] = __builtin_fmaf(from[4 * i] * 0x1p73f, f, o[i]);  // (133 - 60 binades)
+    for (int d0 = 0; d0 < kDB; d0 += kPer) {
+      if (d0 > 0) barrier();
+#pragma unroll
+      for (int d = d0; d < kDB && d < d0 + kPer; ++d) {
+        Vals x;
+        if constexpr (J == 2) {
+          // rows r and r + 8, which are 32 lanes apart, added up: the lower lanes get those of acc[..][2 k], the upper those of
+          // acc[..][2 k + 1]
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float lower = acc[d][2 * k], upper = acc[d][2 * k + 1];
+            const auto y = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, lower),
+                                                            __builtin_bit_cast(unsigned, upper), false, false);
+            const unsigned y0 = y[0], y1 = y[1];
+            x[k] = __builtin_bit_cast(float, y0) + __builtin_bit_cast(float, y1);
           }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] += cr;
-        const int d = 16 * d0 + 4 * dq;
-        if (whole) {
-          const int64_t at = ((int64_t)c.b * p.num_heads + first_head_of(p, v) + hh) * D + d;
-          const float r = 1.f / l;
-          if (p.out_f32)
-            *reinterpret_cast<f32x4 *>(reinterpret_cast<float *>(p.out) + at) = o * r;
-          else
-            *reinterpret_cast<u32x2 *>(reinterpret_cast<uint16_t *>(p.out) + at) =
-                (u32x2){pack_16x2<F16>(o[0] * r, o[1] * r), pack_16x2<F16>(o[2] * r, o[3] * r)};
         } else {
-          const int64_t at = ((int64_t)place * p.chunk_heads + at_hs) * p.group + hh;
-          *reinterpret_cast<f32x4 *>(p.part_o + at * D + d) = o;
-          if (d == 0) *reinterpret_cast<u32x2 *>(p.part_ml + at * 2) = (u32x2){__builtin_bit_cast(unsigned, m), __builtin_bit_cast(unsigned, l)};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) x[k] = acc[d][k];
         }
+        *reinterpret_cast<Vals *>(so + ((wave * kPer + d - d0) * 64 + lane) * kVals) = x;
       }
       barrier();
+      if (head >= 0) {
+#pragma unroll 1
+        for (int d = d0 + rt; d < min(kDB, d0 + kPer); d += tiles) {
+          const float *from = so + ((hs * kPer + d - d0) * 64 + lane) * kVals;
+          Vals o = *reinterpret_cast<const Vals *>(from);
+#pragma unroll 1
+          for (int t = 1; t < tiles; ++t) o += *reinterpret_cast<const Vals *>(from + t * tile_step * kPer * 64 * kVals);
+#pragma unroll
+          for (int k = 0; k < kVals; ++k) {
+            const int row = row_of(k);
+            if (row >= hv) continue;
+            const float x = (o[k] + add[k]) * mul[k];
+            const int64_t at = ((int64_t)c.b * p.num_heads + first_head_of(p, head) + row) * D + 16 * d + n;
+            if (!whole) p.part_o[(part + row) * D + 16 * d + n] = x;
+            else if (p.out_f32) reinterpret_cast<float *>(p.out)[at] = x;
+            else reinterpret_cast<uint16_t *>(p.out)[at] = f32_to_16<F16>(x);
+          }
+        }
+      }
     }
+    barrier();
   };
 
   // ---- the pipeline: while a stage is computed, the next one is on its way
@@ -801,6 +841,7 @@ int plan(DecodeParams &p, int d, int kv_real, size_t &lds) {
     VTKV_REQUIRE(p.row_tiles > 1, "rows of %d bytes leave no room for a stage", p.row_bytes);
   }
   p.min_units = std::max(4, p.row_tiles);
+  p.part_units = 3 * p.row_tiles * kTileRows / kUnitRows;
   return VTKV_OK;
 }
 

@@ -582,7 +582,11 @@ __global__ void __launch_bounds__(kThreads) prefill_attn_kernel(PrefillParams p)
 #pragma unroll
       for (int db = 0; db < kDB; ++db)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) expo = max(expo, __builtin_bit_cast(unsigned, acc[nb][db][i]) & 0x7f800000u);
+        for (int i = 0; i < 4; ++i) {
+          // (a copy first: __builtin_bit_cast of a vector's element gives element 0, whichever is asked for)
+          const float x = acc[nb][db][i];
+          expo = max(expo, __builtin_bit_cast(unsigned, x) & 0x7f800000u);
+        }
     // (one flag at the start of the stage memory, which nobody reads any more: every wave has passed the last
     // stage's barrier; the second pass may only overwrite it once all have read it)
     int *flag = reinterpret_cast<int *>(smem);

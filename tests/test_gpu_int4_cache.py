@@ -355,6 +355,33 @@ def test_prompt_values_beyond_the_fp16_range(env):
     prompt_case(env, 4, [70], [20], 8, 2, v_mul=1e6)
 
 
+@pytest.mark.parametrize("kind", ["bf16", "int4"])
+@pytest.mark.parametrize("column", [0, 1, 2, 3, 6, 61, 127])
+def test_prompt_one_value_beyond_the_fp16_range(env, kind, column):
+    """A single value of V, in whichever column it lies."""
+    torch, ops = env
+    rng = np.random.default_rng(column)
+    n, hq, hkv, d = 50, 4, 2, 128
+    k, v = S.to_bf16(rng.standard_normal((n, hkv, d))), S.to_bf16(rng.standard_normal((n, hkv, d)))
+    v[7, 1, column] = S.to_bf16(np.float64(3e5))
+    r = S.Ranges(1, n, S.row_bytes(hkv, d) if kind == "int4" else 2 * hkv * d)
+    for x, cache in ((k, r.k), (v, r.v)):
+        if kind == "int4":
+            codes = S.quantise(x)
+            x[:] = S.values(*codes)
+            cache[0] = torch.from_numpy(S.pack(*codes)).cuda()
+        else:
+            cache[0] = torch.from_numpy(S.bf16_bits(x).reshape(n, -1).view(np.uint8)).cuda()
+    q, q_host = S.as_type(rng.standard_normal((n, hq, d)), torch.bfloat16)
+    out = torch.full((n, hq, d), 55.0, device="cuda")
+    ops.prefill_attention(out, q, r.kp, r.vp, hkv, d ** -0.5, [n], [n], torch.tensor([0], device="cuda"), None,
+                          "int4" if kind == "int4" else "auto")
+    torch.cuda.synchronize()
+    want = S.attention(q_host, k, v, d ** -0.5, np.arange(n) + 1)
+    # (carried as bfloat16: half a step is 2^-8 of a value; the weights' own rounding a fraction of that)
+    check(out.double().cpu().numpy(), want, np.abs(v).max(), 0.0, 2.0 ** -8)
+
+
 # ------------------------------------------------------------------------------------------------ the paths
 def test_backend_engine_and_step_plan_on_an_int4_cache(env, gpu_pool):
     """Prompts and two decode steps through VTensorImpl over a CacheEngine with kv_cache_dtype="int4", a swap in

@@ -30,8 +30,8 @@
 //    and c * 2^-20; the queries are brought to fp16 by a power of two per wave, exactly, and carry the rest), so S runs on
 //    the fp16 MFMA for either model type; a row's scale and zero, kept beside the stage, turn its dot products into
 //    logits: x = scale (q . c) + zero sum(q).  V is converted on its way in, c * scale + zero in one rounding to fp16
-//    (2^-12 of the value); scales or zeros beyond the fp16 range take the second pass like large bf16 values, there
-//    rounded to bf16.
+//    (2^-12 of the value), the dims in the order in which pairs of codes come out of a word; scales from 128 and zeros
+//    beyond the fp16 range take the second pass like large bf16 values, there rounded to bf16.
 //
 // Otherwise numerics as in the decode kernel (vtkv_attention.hip); the reference computes this with xformers /
 // an external flash-attention kernel (vllm/attention/backends/xformers.py:331-386).
@@ -77,6 +77,7 @@ struct PrefillParams {
   float v_scale;     // 1 for a bf16 cache
 };
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
@@ -106,6 +107,8 @@ __device__ __forceinline__ float wave_max_over_row_groups(float v) {
   swap_rows32(fmax2(a, b), a, b);
   return fmax2(a, b);
 }
+// x as a value the compiler knows nothing about.
+__device__ __forceinline__ void opaque(f32x4 &x) { asm volatile("" : "+v"(x)); }
 // Eight bf16 values (one 16-byte piece of a V row) to eight fp16 values.  Exact for magnitudes in
 // [2^-24, 65504]; a larger one becomes infinity, which makes the unit's result non-finite: the kernel sees that
 // at the end and computes the unit again with V kept in bf16 (see WIDE).
@@ -122,23 +125,25 @@ __device__ __forceinline__ u32x4 codes_to_f16(unsigned w) {
   const unsigned y = w >> 8;
   return (u32x4){w & 0x000f000fu, w & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u};
 }
-// The same codes as values code * s + z in order: fp16 (s, z: the row's scale and zero twice in a register each) or bf16.
+// The same codes as values code * s + z: fp16, in the same order (s: 2^9 times the row's scale, z its zero, twice in a
+// register each), or bf16 pairs in that order.
 __device__ __forceinline__ u32x4 codes_to_values(unsigned w, f16x2 s, f16x2 z) {
-  unsigned v[4];
+  const u32x4 c = codes_to_f16(w);
+  u32x4 v;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const f16x2 c = __builtin_bit_cast(f16x2, ((w >> (4 * i)) & 0x000f000fu) | 0x64006400u) - (f16x2){(_Float16)1024.f, (_Float16)1024.f};
-    v[i] = __builtin_bit_cast(unsigned, __builtin_elementwise_fma(c, s, z));
+  for (int r = 0; r < 4; ++r) {
+    const _Float16 up = r & 1 ? (_Float16)0x1p11f : (_Float16)0x1p15f;  // to c * 2^-9, exactly
+    const unsigned codes = c[r];
+    v[r] = __builtin_bit_cast(unsigned, __builtin_elementwise_fma(__builtin_bit_cast(f16x2, codes) * (f16x2){up, up}, s, z));
   }
-  return (u32x4){__builtin_amdgcn_perm(v[1], v[0], 0x05040100u), __builtin_amdgcn_perm(v[3], v[2], 0x05040100u),
-                 __builtin_amdgcn_perm(v[1], v[0], 0x07060302u), __builtin_amdgcn_perm(v[3], v[2], 0x07060302u)};
+  return v;
 }
 __device__ __forceinline__ u32x4 codes_to_bf16(unsigned w, float s, float z) {
-  u32x4 r;
+  u32x4 v;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    r[i] = pack_bf16x2(__builtin_fmaf((float)((w >> (8 * i)) & 15u), s, z), __builtin_fmaf((float)((w >> (8 * i + 4)) & 15u), s, z));
-  return r;
+  for (int r = 0; r < 4; ++r)
+    v[r] = pack_bf16x2(__builtin_fmaf((float)((w >> (4 * r)) & 15u), s, z), __builtin_fmaf((float)((w >> (4 * r + 16)) & 15u), s, z));
+  return v;
 }
 // KV: what the cache holds, 0 the model's type, 1 e4m3fn codes, 2 4-bit rows.
 // F16: queries, rows and output are fp16 instead of bf16 (rows may still be e4m3fn codes).  S runs on the fp16
@@ -215,7 +220,7 @@ __global__ void __launch_bounds__(kThreads) prefill_attn_kernel(PrefillParams p)
     }
   }
   float sl = p.scale_log2;
-  float q_sum[kNB];  // 4-bit rows: sum(q) in the units of the dot products with the codes
+  float q_sum[kNB];  // 4-bit rows: sum(q)
   if constexpr (I4) {
     float top = 0.f;
 #pragma unroll
@@ -233,14 +238,19 @@ __global__ void __launch_bounds__(kThreads) prefill_attn_kernel(PrefillParams p)
     }
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-    // the power of two that brings the wave's largest query value near 2^14 in fp16
+    float *tops = reinterpret_cast<float *>(smem);
+    if (lane == 0) tops[wave] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, tops[w]);
+    __syncthreads();
+    // the power of two that brings the workgroup's largest query value near 2^14 in fp16
     const int expo = min(max((int)(__builtin_bit_cast(unsigned, top) >> 23), 14), 254);
     const float up = __builtin_bit_cast(float, (unsigned)(268 - expo) << 23);
     const float per_code = up * 0x1p-24f;  // a dot product with the codes over the one with the values 0..15
     sl /= per_code;
 #pragma unroll
     for (int nb = 0; nb < kNB; ++nb) {
-      q_sum[nb] *= per_code;
 #pragma unroll
       for (int ks = 0; ks < kKS; ++ks) {
         float x[8];
@@ -367,13 +377,14 @@ __global__ void __launch_bounds__(kThreads) prefill_attn_kernel(PrefillParams p)
           *reinterpret_cast<u32x4 *>(base + st_v[j]) = codes_to_bf16(vst[j][0], s, z);
           *reinterpret_cast<u32x4 *>(base + (st_v[j] ^ 16)) = codes_to_bf16(vst[j][1], s, z);
         } else {
-          const f16x2 s2 = {(_Float16)s, (_Float16)s}, z2 = {(_Float16)z, (_Float16)z};
+          const _Float16 s16 = (_Float16)(s * 0x1p9f), z16 = (_Float16)z;
+          const f16x2 s2 = {s16, s16}, z2 = {z16, z16};
           *reinterpret_cast<u32x4 *>(base + st_v[j]) = codes_to_values(vst[j][0], s2, z2);
           *reinterpret_cast<u32x4 *>(base + (st_v[j] ^ 16)) = codes_to_values(vst[j][1], s2, z2);
         }
         if (ld_piece[j] == 0) {
-          s_pairs[decltype(bufc)::value][0][ld_row[j]] = __builtin_bit_cast(float, k_pair[j] << 16);
-          s_pairs[decltype(bufc)::value][1][ld_row[j]] = __builtin_bit_cast(float, k_pair[j] & 0xffff0000u);
+          s_pairs[decltype(bufc)::value][0][ld_row[j]] = __builtin_bit_cast(float, k_pair[j] << 16) * sl;
+          s_pairs[decltype(bufc)::value][1][ld_row[j]] = __builtin_bit_cast(float, k_pair[j] & 0xffff0000u) * p.scale_log2;
         }
       } else if constexpr (FP8) {
         // pieces 2p and 2p+1 of a row sit 16 bytes apart before the swizzle, which flips bit 4 or leaves it
@@ -405,7 +416,9 @@ __global__ void __launch_bounds__(kThreads) prefill_attn_kernel(PrefillParams p)
   // accumulators, which otherwise runs whenever any of the wave's 32 columns sees a new maximum, becomes
   // rare.  Without ALiBi the maximum is tracked on the raw dot products (the scale is positive) and the
   // scale is applied inside the exponent's fused multiply-add.
-  const float lazy = ALIBI ? 8.f : 8.f / sl;
+  // 4-bit rows: the logits come relative to the reference point already (the row's scale, its zero and the reference
+  // point are two multiply-adds, the row's numbers carrying the logit scale), and m_run is how far above it they may go.
+  const float lazy = I4 ? 0.f : ALIBI ? 8.f : 8.f / sl;
 
   auto stage = [&](auto bufc, auto widec, int kb) {
     constexpr int buf = decltype(bufc)::value;
@@ -415,6 +428,12 @@ __global__ void __launch_bounds__(kThreads) prefill_attn_kernel(PrefillParams p)
     const int t0 = kb * kKeyBlock;
     if (t0 < wave_end) {  // wave-uniform: else nothing this wave's columns may see
       u32x4 ka[2][kKS];
+      f32x4 row_s[2], row_z[2];  // 4-bit rows: of the rows that this lane's logits belong to
+#pragma unroll
+      for (int t = 0; t < 2 && I4; ++t) {
+        row_s[t] = *reinterpret_cast<const f32x4 *>(&s_pairs[buf][0][16 * t + 4 * g]);
+        row_z[t] = *reinterpret_cast<const f32x4 *>(&s_pairs[buf][1][16 * t + 4 * g]);
+      }
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -437,20 +456,6 @@ __global__ void __launch_bounds__(kThreads) prefill_attn_kernel(PrefillParams p)
           for (int ks = 0; ks < kKS; ++ks)
             sacc[nb][t] = mfma_16x16x32<SF16>(ka[t][ks], qop[nb][ks], sacc[nb][t]);
         }
-      if constexpr (I4) {  // dot products with codes to dot products with values (in units of the former)
-        f32x4 ks[2], kz[2];
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          ks[t] = *reinterpret_cast<const f32x4 *>(&s_pairs[buf][0][16 * t + 4 * g]);
-          kz[t] = *reinterpret_cast<const f32x4 *>(&s_pairs[buf][1][16 * t + 4 * g]);
-        }
-#pragma unroll
-        for (int nb = 0; nb < kNB; ++nb)
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) sacc[nb][t][r] = __builtin_fmaf(ks[t][r], sacc[nb][t][r], kz[t][r] * q_sum[nb]);
-      }
       // reduction slot (g, j) of the K=32 P.V MFMA stands for row 4g+j of the first tile (j < 4) and row
       // 4g+j-4 of the second (j >= 4), so a lane's A operand is its transposed quad of the first tile
       // followed by that of the second; read once for both column blocks
@@ -468,13 +473,17 @@ __global__ void __launch_bounds__(kThreads) prefill_attn_kernel(PrefillParams p)
 #pragma unroll
       for (int nb = 0; nb < kNB; ++nb) {
         // x[4t + r] belongs to row t0 + 16t + 4g + r of the lane's column: with ALiBi the logit in log2
-        // units, else the raw dot product
+        // units, else the raw dot product; of 4-bit rows always the logit in log2 units above the reference point
         float x[8];
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            if (ALIBI)
+            if constexpr (I4) {
+              const float above = ALIBI ? __builtin_fmaf(slope_log2[nb], (float)(t0 + 16 * t + 4 * g + r - limit[nb] + 1), m_off[nb])
+                                        : m_off[nb];
+              x[4 * t + r] = __builtin_fmaf(row_s[t][r], sacc[nb][t][r], __builtin_fmaf(row_z[t][r], q_sum[nb], above));
+            } else if (ALIBI)
               x[4 * t + r] = __builtin_fmaf(sacc[nb][t][r], sl,
                                             slope_log2[nb] * (float)(t0 + 16 * t + 4 * g + r - limit[nb] + 1));
             else
@@ -493,19 +502,33 @@ __global__ void __launch_bounds__(kThreads) prefill_attn_kernel(PrefillParams p)
         if (__builtin_amdgcn_ballot_w64(lmax > m_run[nb] + lazy) != 0) {  // rare: some column moves its reference point
           const float tmax = wave_max_over_row_groups(lmax);
           const bool grow = tmax > m_run[nb] + lazy;
-          const float m_new = grow ? tmax : m_run[nb];
-          // (a column that has seen only masked rows keeps -inf and rescales its zeros by 1)
-          const float alpha = grow ? __builtin_amdgcn_exp2f(ALIBI ? m_run[nb] - m_new : (m_run[nb] - m_new) * sl) : 1.f;
-          m_run[nb] = m_new;
-          // (a column can have everything so far masked; the reference point 0 keeps exp2(-inf - ref) = 0)
-          const float m_ref = m_new == -INFINITY ? 0.f : m_new;
-          m_off[nb] = ALIBI ? -m_ref : -m_ref * sl;
+          float alpha;
+          if constexpr (I4) {
+            // (a column's first logit finds zeros in its accumulators; all masked so far: the reference point stays 0)
+            const float up = grow ? tmax : 0.f;
+            alpha = m_run[nb] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(-up);
+            m_run[nb] = grow ? 8.f : m_run[nb];
+            m_off[nb] -= up;
+#pragma unroll
+            for (int r = 0; r < 8; ++r) x[r] -= up;
+          } else {
+            const float m_new = grow ? tmax : m_run[nb];
+            // (a column that has seen only masked rows keeps -inf and rescales its zeros by 1)
+            alpha = grow ? __builtin_amdgcn_exp2f(ALIBI ? m_run[nb] - m_new : (m_run[nb] - m_new) * sl) : 1.f;
+            m_run[nb] = m_new;
+            // (a column can have everything so far masked; the reference point 0 keeps exp2(-inf - ref) = 0)
+            const float m_ref = m_new == -INFINITY ? 0.f : m_new;
+            m_off[nb] = ALIBI ? -m_ref : -m_ref * sl;
+          }
           acc_l[nb] *= alpha;
 #pragma unroll
           for (int d = 0; d < kDB; ++d) acc[nb][d] *= alpha;
         }
         float pr[8];
-        if (ALIBI) {
+        if constexpr (I4) {
+#pragma unroll
+          for (int r = 0; r < 8; ++r) pr[r] = __builtin_amdgcn_exp2f(x[r]);
+        } else if (ALIBI) {
 #pragma unroll
           for (int r = 0; r < 8; ++r) pr[r] = __builtin_amdgcn_exp2f(x[r] + m_off[nb]);
         } else {
@@ -566,6 +589,14 @@ __global__ void __launch_bounds__(kThreads) prefill_attn_kernel(PrefillParams p)
       stage(std::integral_constant<int, 0>{}, widec, kb);
       if (kb + 1 < nblocks) stage(std::integral_constant<int, 1>{}, widec, kb + 1);
     }
+    // (the results as values the compiler knows nothing about: else the two passes' accumulators are one web, and it keeps
+    // them in two sets of registers with a copy of all of them in every stage)
+#pragma unroll
+    for (int nb = 0; nb < kNB; ++nb) {
+      opaque(acc_l[nb]);
+#pragma unroll
+      for (int db = 0; db < kDB; ++db) opaque(acc[nb][db]);
+    }
   };
   run(std::false_type{});
 #ifdef VTKV_PREFILL_TRACE
@@ -603,21 +634,36 @@ __global__ void __launch_bounds__(kThreads) prefill_attn_kernel(PrefillParams p)
     }
   }
 
-  // ---- normalise and store: lane (n, g) holds O[column n][d = 16*db + 4g + i]
+  // ---- normalise and store: lane (n, g) holds O[column n][place 16*db + 4g + i].  A place is its dim, except with 4-bit rows:
+  // place q of eight is dim q / 2 + 4 (q & 1) of them, so the lane has two pairs of neighbouring dims, four apart.
 #pragma unroll
   for (int nb = 0; nb < kNB; ++nb) {
     const float l = acc_l[nb][0];  // (already the sum over all rows: see acc_l)
     if (col_tok[nb] < 0) continue;
     const float inv = p.v_scale / l;
-    const int64_t o0 = ((int64_t)(u_row0 + col_tok[nb]) * p.num_heads + head0 + col_head[nb]) * kD + 4 * g;
+    const int64_t o0 = ((int64_t)(u_row0 + col_tok[nb]) * p.num_heads + head0 + col_head[nb]) * kD +
+                       (I4 ? 8 * (g >> 1) + 2 * (g & 1) : 4 * g);
 #pragma unroll
     for (int db = 0; db < kDB; ++db) {
-      const f32x4 r = acc[nb][db] * inv;
+      f32x4 r = acc[nb][db] * inv;
+      if constexpr (I4) r = (f32x4){r[0], r[2], r[1], r[3]};
       if (p.out_f32) {
-        *reinterpret_cast<f32x4 *>(reinterpret_cast<float *>(p.out) + o0 + db * 16) = r;
+        float *to = reinterpret_cast<float *>(p.out) + o0 + db * 16;
+        if constexpr (I4) {
+          *reinterpret_cast<f32x2 *>(to) = (f32x2){r[0], r[1]};
+          *reinterpret_cast<f32x2 *>(to + 4) = (f32x2){r[2], r[3]};
+        } else {
+          *reinterpret_cast<f32x4 *>(to) = r;
+        }
       } else {
         u32x2 w = {pack_16x2<F16>(r[0], r[1]), pack_16x2<F16>(r[2], r[3])};
-        *reinterpret_cast<u32x2 *>(reinterpret_cast<uint16_t *>(p.out) + o0 + db * 16) = w;
+        uint16_t *to = reinterpret_cast<uint16_t *>(p.out) + o0 + db * 16;
+        if constexpr (I4) {
+          *reinterpret_cast<unsigned *>(to) = w[0];
+          *reinterpret_cast<unsigned *>(to + 4) = w[1];
+        } else {
+          *reinterpret_cast<u32x2 *>(to) = w;
+        }
       }
     }
   }

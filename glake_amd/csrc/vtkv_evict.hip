@@ -49,6 +49,17 @@ __device__ __forceinline__ void load_to_lds(uint64_t base, uint32_t off, uint32_
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds), "v"(off), "s"(base) : "memory");
 }
 
+// A maximum as one instruction (fmaxf() first quiets operands that the compiler cannot prove canonical).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+// The value of the lane eight places on in its sixteen.
+__device__ __forceinline__ float other_part(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x128, 0xf, 0xf, true));
+}
+
 // KV: 0: 16-bit rows of the model's type, 1: e4m3fn codes, 2: 4-bit rows.  A wave takes up to kTiles tiles of 64 rows
 // of one kv head one after the other; while a tile is multiplied, the next one is on its way.  The workgroup's waves take
 // kv heads next to each other of the same rows, since a head's part of a row is short (64 sequences of 512 to 4096 rows,
@@ -58,11 +69,13 @@ __device__ __forceinline__ void load_to_lds(uint64_t base, uint32_t off, uint32_
 //    from there into registers, which frees the LDS for the next tile.  Rows of a power of two of 16-byte pieces have their
 //    pieces exchanged by row so that operand reads meet all banks.  Two tiles per wave: 68 us, one 78, four 74, eight 71.
 //  * 4-bit codes go straight into operand registers and are multiplied as fp16 denormals, q carrying the rest, and a row's
-//    scale and zero applied to its logits (as in vtkv_int4_decode.hip).  29 us for 24
+//    scale and zero applied to its logits (as in vtkv_int4_decode.hip).  27 us for 24
 //    sequences of 1024 to 8192 rows and 64 query heads over 8 kv heads, one tile per wave or two.
 constexpr int kTiles = 2;
 
-template <int D, int KV, bool F16>
+// J = 2: up to eight query heads per kv head: a lane's column is (part j, head), and of two 16-row tiles it keeps the logits
+// of the j-th, so that what follows the products is done once per logit (J = 1 for the 24 sequences above: 29 us instead of 27).
+template <int D, int KV, bool F16, int J>
 __global__ void __launch_bounds__(KV == 2 ? 512 : 256) attention_logits_kernel(WeightParams p) {
   constexpr bool I4 = KV == 2, FP8 = KV == 1;
   constexpr int kWords = D / 8;                                                // 4-bit rows: words of eight codes
@@ -73,7 +86,8 @@ __global__ void __launch_bounds__(KV == 2 ? 512 : 256) attention_logits_kernel(W
   constexpr int kSteps = FP8 ? 2 * kPieces : (kWords + 3) / 4;                 // MFMA steps over d
   __shared__ __attribute__((aligned(16))) char s_rows[I4 ? 1 : 4][I4 ? 16 : kTileRows * kHeadBytes];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), waves = blockDim.x >> 6;
-  const int g = lane >> 4, n = lane & 15;
+  constexpr int kHeads = 16 / J, kE = 4 / J;
+  const int g = lane >> 4, n = lane & 15, j = n / kHeads, h = n % kHeads;
   const int b = blockIdx.z, groups = (p.num_kv_heads + p.heads_wg - 1) / p.heads_wg;
   const int v = blockIdx.x % groups * p.heads_wg + wave % p.heads_wg;
   const int first = (blockIdx.x / groups * (waves / p.heads_wg) + wave / p.heads_wg) * kTiles * kTileRows;
@@ -130,11 +144,11 @@ __global__ void __launch_bounds__(KV == 2 ? 512 : 256) attention_logits_kernel(W
   u32x4 qop[kSteps];
   float q_back = p.scale_log2, q_sum = 0.f;
   {
-    const uint16_t *q_row = p.q + (int64_t)b * p.q_stride + (int64_t)(h0 + min(n, hv - 1)) * D;
+    const uint16_t *q_row = p.q + (int64_t)b * p.q_stride + (int64_t)(h0 + min(h, hv - 1)) * D;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       const int at = I4 ? 8 * (word0 + s) : FP8 ? 16 * (4 * (s / 2) + g) + 8 * (s & 1) : 8 * (4 * s + g);
-      const bool live = n < hv && (I4 ? s < words : at < D);
+      const bool live = h < hv && (I4 ? s < words : at < D);
       qop[s] = (u32x4){0, 0, 0, 0};
       if (live) qop[s] = *reinterpret_cast<const u32x4 *>(q_row + at);
     }
@@ -167,7 +181,8 @@ __global__ void __launch_bounds__(KV == 2 ? 512 : 256) attention_logits_kernel(W
       }
     }
   }
-  const float slope = p.alibi_slopes && n < hv ? p.alibi_slopes[h0 + n] * kLog2e : 0.f;
+  const float slope = p.alibi_slopes && h < hv ? p.alibi_slopes[h0 + h] * kLog2e : 0.f;
+  const int row_at = 16 * (J == 2 ? j : 0) + 4 * g;  // this lane's rows of a tile: 16 J e + row_at + i
 
 #pragma unroll 1
   for (int row0 = first; row0 < last; row0 += kTileRows) {
@@ -188,52 +203,71 @@ __global__ void __launch_bounds__(KV == 2 ? 512 : 256) attention_logits_kernel(W
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
     if (more) ask(row0 + kTileRows, next);
-    // ---- logits: lane (n, g) holds rows 16 t + 4 g + i of head n
-    f32x4 x[4];
-    float top = -INFINITY;
+    // ---- logits
+    f32x4 x[kE];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      f32x4 a = {0.f, 0.f, 0.f, 0.f};
+    for (int e = 0; e < kE; ++e) {
+      f32x4 a[J];
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        if constexpr (I4) {
-          const unsigned w = now.w[t][s], y = w >> 8;
-          a = mfma_16x16x32<true>((u32x4){w & 0x000f000fu, w & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u}, qop[s], a);
-        } else if constexpr (FP8) {
-          a = mfma_16x16x32<F16>(fp8x8_widen<F16>(kr[t][s / 2][2 * (s & 1)], kr[t][s / 2][2 * (s & 1) + 1]), qop[s], a);
-        } else {
-          a = mfma_16x16x32<F16>(kr[t][s], qop[s], a);
+      for (int q = 0; q < J; ++q) {
+        const int t = J * e + q;
+        a[q] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+          if constexpr (I4) {
+            const unsigned w = now.w[t][s], y = w >> 8;
+            a[q] = mfma_16x16x32<true>((u32x4){w & 0x000f000fu, w & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u}, qop[s], a[q]);
+          } else if constexpr (FP8) {
+            a[q] = mfma_16x16x32<F16>(fp8x8_widen<F16>(kr[t][s / 2][2 * (s & 1)], kr[t][s / 2][2 * (s & 1) + 1]), qop[s], a[q]);
+          } else {
+            a[q] = mfma_16x16x32<F16>(kr[t][s], qop[s], a[q]);
+          }
         }
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int row = 16 * t + 4 * g + i;
+        const float dot = J == 2 ? (j == 0 ? a[0][i] : a[J - 1][i]) : a[0][i];
         if constexpr (I4) {
-          const unsigned sz = (unsigned)__shfl((int)now.pair, row);
-          a[i] = __builtin_fmaf(__builtin_bit_cast(float, sz << 16) * a[i], q_back, __builtin_bit_cast(float, sz & 0xffff0000u) * q_sum);
+          const unsigned sz = (unsigned)__shfl((int)now.pair, 16 * J * e + row_at + i);
+          x[e][i] = __builtin_fmaf(__builtin_bit_cast(float, sz << 16) * dot, q_back, __builtin_bit_cast(float, sz & 0xffff0000u) * q_sum);
         } else {
-          a[i] *= q_back;
+          x[e][i] = dot * q_back;
         }
-        a[i] = __builtin_fmaf(slope, (float)(row0 + row - len + 1), a[i]);
-        if (row >= rows) a[i] = -INFINITY;
-        top = fmaxf(top, a[i]);
       }
-      x[t] = a;
     }
+    if (p.alibi_slopes) {
+      const float ahead = (float)(row0 + row_at - len + 1);
+#pragma unroll
+      for (int e = 0; e < kE; ++e)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[e][i] = __builtin_fmaf(slope, ahead + (float)(16 * J * e + i), x[e][i]);
+    }
+    if (rows < kTileRows) {
+#pragma unroll
+      for (int e = 0; e < kE; ++e)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (16 * J * e + row_at + i >= rows) x[e][i] = -INFINITY;
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < kE; ++e) top = max3(max3(top, x[e][0], x[e][1]), x[e][2], x[e][3]);
     top = max_over_row_groups(top);
+    if constexpr (J == 2) top = max3(top, other_part(top), top);
     const float ref = top == -INFINITY ? 0.f : top;
     float sum = 0.f;
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int e = 0; e < kE; ++e)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum += __builtin_amdgcn_exp2f(x[t][i] - ref);
+      for (int i = 0; i < 4; ++i) sum += __builtin_amdgcn_exp2f(x[e][i] - ref);
     sum = sum_over_row_groups(sum);
-    if (n < hv) {
-      const int64_t head = (int64_t)b * p.num_heads + h0 + n;
-      float *to = p.logits + head * p.pitch + row0 + 4 * g;
+    if constexpr (J == 2) sum += other_part(sum);
+    if (h < hv) {
+      const int64_t head = (int64_t)b * p.num_heads + h0 + h;
+      float *to = p.logits + head * p.pitch + row0 + row_at;
 #pragma unroll
-      for (int t = 0; t < 4; ++t) *reinterpret_cast<f32x4 *>(to + 16 * t) = x[t];
-      if (g == 0) *reinterpret_cast<u32x2 *>(p.stats + (head * (p.pitch / kTileRows) + row0 / kTileRows) * 2) =
+      for (int e = 0; e < kE; ++e) *reinterpret_cast<f32x4 *>(to + 16 * J * e) = x[e];
+      if (g == 0 && j == 0) *reinterpret_cast<u32x2 *>(p.stats + (head * (p.pitch / kTileRows) + row0 / kTileRows) * 2) =
           (u32x2){__builtin_bit_cast(unsigned, top), __builtin_bit_cast(unsigned, sum)};
     }
   }
@@ -302,13 +336,20 @@ __global__ void __launch_bounds__(kSumThreads) add_weights_kernel(WeightParams p
     if (row + i < len) w[i] += acc[i];
 }
 
-template <int D>
+template <int D, int J>
 void launch_logits(const WeightParams &p, int kv, bool f16, dim3 grid, int threads, hipStream_t st) {
   typedef void (*Kernel)(WeightParams);
-  static const Kernel kernels[3][2] = {{attention_logits_kernel<D, 0, false>, attention_logits_kernel<D, 0, true>},
-                                       {attention_logits_kernel<D, 1, false>, attention_logits_kernel<D, 1, true>},
-                                       {attention_logits_kernel<D, 2, false>, attention_logits_kernel<D, 2, true>}};
+  static const Kernel kernels[3][2] = {{attention_logits_kernel<D, 0, false, J>, attention_logits_kernel<D, 0, true, J>},
+                                       {attention_logits_kernel<D, 1, false, J>, attention_logits_kernel<D, 1, true, J>},
+                                       {attention_logits_kernel<D, 2, false, J>, attention_logits_kernel<D, 2, true, J>}};
   hipLaunchKernelGGL(kernels[kv][f16], grid, dim3((unsigned)threads), 0, st, p);
+}
+template <int D>
+void launch_logits(const WeightParams &p, int kv, bool f16, dim3 grid, int threads, hipStream_t st) {
+  if (p.group <= 8)
+    launch_logits<D, 2>(p, kv, f16, grid, threads, st);
+  else
+    launch_logits<D, 1>(p, kv, f16, grid, threads, st);
 }
 
 int64_t weight_pitch(int max_seq_len) { return ((int64_t)max_seq_len + kTileRows - 1) / kTileRows * kTileRows; }

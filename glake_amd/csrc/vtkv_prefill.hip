@@ -194,7 +194,8 @@ __global__ void __launch_bounds__(kThreads) prefill_attn_kernel(PrefillParams p)
   const uint32_t row_stride = I4 ? (uint32_t)p.row_bytes : (uint32_t)(Hkv / p.kv_split) * kKvRowBytes;
   // 4-bit rows: from a head's codes to its scale and zero
   const uint32_t to_pair = (uint32_t)(Hkv / p.kv_split - kv_real) * kKvRowBytes + 4 * kv_real;
-  __shared__ float s_pairs[I4 ? 2 : 1][2][I4 ? kKeyBlock : 1];  // per stage: the K rows' scales, then their zeros
+  // per stage: the K rows' scales, then their zeros, then (second pass) which V rows are not finite
+  __shared__ float s_pairs[I4 ? 2 : 1][3][I4 ? kKeyBlock : 1];
   const int head0 = first_head_of(p, kvh), n_heads = heads_of(p, kvh);
 
   // ---- this wave's columns: block nb, column n -> (token, head); unused columns get q = 0
@@ -279,11 +280,13 @@ __global__ void __launch_bounds__(kThreads) prefill_attn_kernel(PrefillParams p)
   // the reference point it follows.
   f32x4 acc_l[kNB];
   float m_run[kNB], m_off[kNB];
+  float sees_bad[kNB];  // 4-bit rows, second pass: the column sees a V row that is not finite
   auto reset = [&]() {
 #pragma unroll
     for (int nb = 0; nb < kNB; ++nb) {
       m_run[nb] = -INFINITY;
       m_off[nb] = 0.f;
+      sees_bad[nb] = 0.f;
       acc_l[nb] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < kDB; ++i) acc[nb][i] = (f32x4){0.f, 0.f, 0.f, 0.f};
@@ -374,8 +377,13 @@ __global__ void __launch_bounds__(kThreads) prefill_attn_kernel(PrefillParams p)
       if constexpr (I4) {
         *reinterpret_cast<u32x4 *>(base + st_k[j]) = codes_to_f16(kst[j][0]);
         *reinterpret_cast<u32x4 *>(base + (st_k[j] ^ 16)) = codes_to_f16(kst[j][1]);
-        const float s = __builtin_bit_cast(float, v_pair[j] << 16), z = __builtin_bit_cast(float, v_pair[j] & 0xffff0000u);
+        float s = __builtin_bit_cast(float, v_pair[j] << 16), z = __builtin_bit_cast(float, v_pair[j] & 0xffff0000u);
         if constexpr (WIDE) {
+          // a row that is not finite counts as zeros here and makes the columns that see it NaN in the end: a weight of zero
+          // times NaN would do that to those that do not
+          const bool bad = (v_pair[j] & 0x7f80u) == 0x7f80u || (v_pair[j] & 0x7f800000u) == 0x7f800000u;
+          if (bad) s = z = 0.f;
+          if (ld_piece[j] == 0) s_pairs[decltype(bufc)::value][2][ld_row[j]] = bad ? 1.f : 0.f;
           *reinterpret_cast<u32x4 *>(base + st_v[j]) = codes_to_bf16(vst[j][0], s, z);
           *reinterpret_cast<u32x4 *>(base + (st_v[j] ^ 16)) = codes_to_bf16(vst[j][1], s, z);
         } else {
@@ -497,6 +505,13 @@ __global__ void __launch_bounds__(kThreads) prefill_attn_kernel(PrefillParams p)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
               if (t0 + 16 * t + 4 * g + r >= limit[nb]) x[4 * t + r] = -INFINITY;
+        }
+        if constexpr (I4 && WIDE) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (x[4 * t + r] != -INFINITY) sees_bad[nb] = fmaxf(sees_bad[nb], s_pairs[buf][2][16 * t + 4 * g + r]);
         }
         // the lane's own maximum; the maximum of the column (its four row groups) is only needed when some lane
         // sees a value above the reference point's margin, which is exactly when the column's maximum is above it
@@ -641,8 +656,9 @@ __global__ void __launch_bounds__(kThreads) prefill_attn_kernel(PrefillParams p)
 #pragma unroll
   for (int nb = 0; nb < kNB; ++nb) {
     const float l = acc_l[nb][0];  // (already the sum over all rows: see acc_l)
+    float inv = p.v_scale / l;
+    if (I4 && wave_max_over_row_groups(sees_bad[nb]) > 0.f) inv = __builtin_nanf("");
     if (col_tok[nb] < 0) continue;
-    const float inv = p.v_scale / l;
     const int64_t o0 = ((int64_t)(u_row0 + col_tok[nb]) * p.num_heads + head0 + col_head[nb]) * kD +
                        (I4 ? 8 * (g >> 1) + 2 * (g & 1) : 4 * g);
 #pragma unroll

@@ -222,6 +222,66 @@ def test_decode_many_and_long_sequences(env):
     decode_case(env, 7, [9001, 5], 4, 1, 256)
 
 
+def test_decode_ragged_batches(env):
+    """Sequences of a few rows between empty and long ones: workgroups with several sequences, spans that begin or end before
+    a sequence's first row."""
+    rng = np.random.default_rng(14)
+    decode_case(env, 15, [1] * 70, 8, 8, 80)
+    decode_case(env, 16, [0, 1] * 60 + [3000], 8, 2)
+    decode_case(env, 17, list(rng.integers(0, 300, 40)) + [9000] + list(rng.integers(0, 20, 40)), 16, 16, 64, "fp16")
+    decode_case(env, 18, list(rng.integers(1, 600, 33)), 24, 1, 128)
+
+
+@pytest.mark.parametrize("factor", [1e6, 1e-12])
+def test_decode_large_and_small_values(env, factor):
+    torch, ops = env
+    rng = np.random.default_rng(19)
+    lens, hq, hkv, d = [200, 33], 8, 2, 128
+    r, k, v = filled(rng, lens, hkv, d, [0, 1])
+    for i, n in enumerate(lens):
+        x = S.quantise(S.to_bf16(factor * S.model_values(rng, (n, hkv, d))))
+        v[i] = S.values(*x)
+        r.v[i, :n] = torch.from_numpy(S.pack(*x)).cuda()
+    q, q_host = S.as_type(rng.standard_normal((2, hq, d)) * 1.5, torch.bfloat16)
+    out = torch.full((2, hq, d), 55.0, device="cuda")
+    ops.paged_attention_v1(out, q, r.kp, r.vp, hkv, d ** -0.5, torch.tensor(lens, dtype=torch.int32, device="cuda"), 1, 200,
+                           None, "int4", 1.0, torch.tensor([0, 1], device="cuda"))
+    for i in range(2):
+        want = S.attention(q_host[i:i + 1], k[i], v[i], d ** -0.5)[0]
+        # (weights times scales below 2^-57 lose bits, 2^-53 at most per row)
+        check(out[i].double().cpu().numpy() / factor, want / factor, np.abs(v[i]).max() / factor, 0.0,
+              2.0 ** -12 + lens[i] * 15 * 2.0 ** -53 / np.abs(v[i]).max())
+
+
+def test_decode_without_a_workspace(env):
+    """The entry point that takes no workspace, against the one that does."""
+    import ctypes as C
+
+    from glake_amd import _C
+
+    torch, _ = env
+    rng = np.random.default_rng(20)
+    for lens, hq, hkv, d in (([700, 1, 33, 0, 5000], 32, 8, 128), ([90, 400], 128, 8, 256)):
+        b = len(lens)
+        r, _, _ = filled(rng, lens, hkv, d, list(range(b)))
+        q = torch.from_numpy(rng.standard_normal((b, hq, d)).astype(np.float32)).bfloat16().cuda()
+        lens_t = torch.tensor(lens, dtype=torch.int32, device="cuda")
+        slots = torch.arange(b, device="cuda")
+        outs = [torch.full((b, hq, d), 55.0, device="cuda") for _ in range(2)]
+        lib = _C.lib()
+        p = lambda t: C.c_void_p(t.data_ptr())  # noqa: E731
+        stream = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+        ws = torch.zeros(lib.vtkv_decode_attention_workspace_bytes(b, hq, d, max(lens), 0), dtype=torch.uint8, device="cuda")
+        for out, tail, entry in ((outs[0], (), lib.vtkv_decode_attention_noalloc),
+                                 (outs[1], (p(ws), ws.numel(), 0), lib.vtkv_decode_attention)):
+            _C.check(entry(p(out), p(q), p(r.kp), p(r.vp), p(slots), p(lens_t), b, hq, hkv, d, hq * d, d ** -0.5, max(lens), None,
+                           _C.BF16, _C.F32, _C.INT4, 1.0, 1.0, *tail, stream))
+        torch.cuda.synchronize()
+        # (the spans may differ with the workspace, and with them the order of the sums: 2^-12 of the values each)
+        assert torch.isfinite(outs[0]).all() and (outs[0] - outs[1]).abs().max() <= 2.0 ** -11 * 10
+        assert (outs[0][3] == 0).all() if len(lens) == 5 else True
+
+
 def test_decode_strided_queries(env):
     torch, ops = env
     rng = np.random.default_rng(11)
@@ -355,6 +415,11 @@ def test_prompt_values_beyond_the_fp16_range(env):
     prompt_case(env, 4, [70], [20], 8, 2, v_mul=1e6)
 
 
+def test_prompt_scales_from_128_on(env):
+    prompt_case(env, 6, [70, 40], [20, 0], 8, 2, v_mul=1e3)
+    prompt_case(env, 7, [40], [0], 8, 2, dtype="fp16", v_mul=1e3)
+
+
 @pytest.mark.parametrize("kind", ["bf16", "int4"])
 @pytest.mark.parametrize("column", [0, 1, 2, 3, 6, 61, 127])
 def test_prompt_one_value_beyond_the_fp16_range(env, kind, column):
@@ -380,6 +445,30 @@ def test_prompt_one_value_beyond_the_fp16_range(env, kind, column):
     want = S.attention(q_host, k, v, d ** -0.5, np.arange(n) + 1)
     # (carried as bfloat16: half a step is 2^-8 of a value; the weights' own rounding a fraction of that)
     check(out.double().cpu().numpy(), want, np.abs(v).max(), 0.0, 2.0 ** -8)
+
+
+@pytest.mark.parametrize("side", ["k", "v"])
+def test_prompt_a_row_that_is_not_finite_stays_with_the_tokens_that_see_it(env, side):
+    torch, ops = env
+    rng = np.random.default_rng(31)
+    query_lens, cached, hq, hkv, d, bad = [90, 50], [0, 40], 8, 2, 128, 61
+    lens = [a + c for a, c in zip(query_lens, cached)]
+    r, k, v = filled(rng, lens, hkv, d, [1, 0])
+    cache = r.k if side == "k" else r.v
+    cache[0, bad, hkv * d // 2 + 4:hkv * d // 2 + 8] = torch.tensor([0xC0, 0x7F, 0xC0, 0x7F], dtype=torch.uint8)  # head 1
+    q, q_host = S.as_type(rng.standard_normal((sum(query_lens), hq, d)), torch.bfloat16)
+    out = torch.full((sum(query_lens), hq, d), 55.0, device="cuda")
+    ops.prefill_attention(out, q, r.kp, r.vp, hkv, d ** -0.5, query_lens, lens, torch.tensor([1, 0], device="cuda"), None, "int4")
+    out = out.double().cpu().numpy()
+    sees = bad - cached[1]  # the first token of the second sequence that sees the row
+    assert np.isnan(out[90 + sees:, 4:]).all()
+    for i, at in ((0, 0), (1, 90)):
+        want = S.attention(q_host[at:at + query_lens[i]], k[i], v[i], d ** -0.5, np.arange(cached[i], lens[i]) + 1)
+        got = out[at:at + query_lens[i]]
+        v_max = np.abs(v[i]).max()
+        # (the tokens before it may have been computed with bfloat16 values: half a step is 2^-8 of a value)
+        check(got[:, :4], want[:, :4], v_max, 0.0, 2.0 ** -8)
+        check(got[:sees if i else None, 4:], want[:sees if i else None, 4:], v_max, 0.0, 2.0 ** -8)
 
 
 # ------------------------------------------------------------------------------------------------ the paths

@@ -84,6 +84,18 @@ def _on_current_device(*tensors) -> None:
                 raise _C.VtkvError(_C.EINVAL, f"tensor on {t.device}, but the current device is {here}")
 
 
+def _pointer_tables(*tables) -> None:
+    """Base addresses per slot as the kernels read them (a raw integer address is taken as it is)."""
+    for t in tables:
+        if isinstance(t, torch.Tensor) and not (t.is_cuda and t.dtype == torch.int64 and t.is_contiguous()):
+            raise _C.VtkvError(_C.EINVAL, "a pointer table must be int64 and contiguous, on the GPU")
+
+
+def _num_slots(weights: torch.Tensor, *tables) -> int:
+    """Slots that the weights and every pointer table have (a slot beyond them is skipped)."""
+    return min([weights.shape[0]] + [t.numel() for t in tables if isinstance(t, torch.Tensor)])
+
+
 def _slopes(alibi_slopes: Optional[torch.Tensor], num_heads: int, device: torch.device) -> Optional[torch.Tensor]:
     if alibi_slopes is None:
         return None
@@ -161,6 +173,7 @@ def paged_attention_v1(
         _int4_scales(kv_cache_dtype, kv_scale, v_scale)
         _per_sequence(num_seqs, seq_lens, slot_mapping)
         _on_current_device(out, query, key_cache, value_cache, seq_lens, slot_mapping)
+        _pointer_tables(key_cache, value_cache)
         _int4_query(out, query)
         alibi_slopes = _slopes(alibi_slopes, num_heads, query.device)
     if seq_lens.dtype != torch.int32 or slot_mapping.dtype != torch.int64:
@@ -299,6 +312,7 @@ def prefill_attention(
     if kv_cache_dtype == "int4":
         _int4_scales(kv_cache_dtype, kv_scale, v_scale)
         _on_current_device(out, query, key_cache, value_cache, slot_mapping)
+        _pointer_tables(key_cache, value_cache)
         _int4_query(out, query)
         alibi_slopes = _slopes(alibi_slopes, query.shape[1], query.device)
         if slot_mapping.shape[0] < len(seq_lens) or not slot_mapping.is_contiguous():
@@ -413,6 +427,7 @@ def reshape_and_cache(
     if kv_cache_dtype == "int4":
         _int4_scales(kv_cache_dtype, k_scale, v_scale)
         _require_cuda(seq_lens, cache_seq_lens)
+        _pointer_tables(key_cache, value_cache)
         _on_current_device(key, value, key_cache, value_cache, slot_m, slot_mapping, seq_lens, cache_seq_lens)
         if any(t is not None and not t.is_contiguous() for t in (seq_lens, cache_seq_lens)):
             raise _C.VtkvError(_C.EINVAL, "seq_lens and cache_seq_lens must be contiguous")
@@ -457,6 +472,7 @@ def read_cached_rows(
     if kv_cache_dtype != "int4":
         raise _C.VtkvError(_C.EINVAL, f"read_cached_rows reads int4 caches, not {kv_cache_dtype}")
     _require_cuda(key, value, slot_m, slot_mapping, seq_lens, cache_seq_lens)
+    _pointer_tables(key_cache, value_cache)
     _on_current_device(key, value, key_cache, value_cache, slot_m, slot_mapping, seq_lens, cache_seq_lens)
     if slot_m.dtype != torch.int64 or slot_mapping.dtype != torch.int64 or slot_m.shape != slot_mapping.shape:
         raise _C.VtkvError(_C.EINVAL, "slot_m and slot_mapping must be int64, one entry per sequence")
@@ -504,6 +520,7 @@ def accumulate_attention_weights(
     _per_sequence(num_seqs, seq_lens, slot_mapping)
     _weights_of(weights, num_kv_heads, max_seq_len)
     _on_current_device(weights, query, key_cache, seq_lens, slot_mapping)
+    _pointer_tables(key_cache)
     if query.stride(2) != 1 or query.stride(1) != head_size:
         raise _C.VtkvError(_C.EINVAL, "query rows must be contiguous in (head, dim)")
     _int4_scales(kv_cache_dtype, kv_scale)
@@ -512,7 +529,7 @@ def accumulate_attention_weights(
     alibi_slopes = _slopes(alibi_slopes, num_heads, query.device)
     ws = _scratch(lib.vtkv_accumulate_attention_weights_workspace_bytes(num_seqs, num_heads, max_seq_len), query.device)
     _C.check(lib.vtkv_accumulate_attention_weights(
-        _ptr(weights), weights.stride(0), weights.stride(1), weights.shape[0], _ptr(query), _ptr(key_cache),
+        _ptr(weights), weights.stride(0), weights.stride(1), _num_slots(weights, key_cache), _ptr(query), _ptr(key_cache),
         _ptr(slot_mapping), _ptr(seq_lens), num_seqs, num_heads, num_kv_heads, head_size, query.stride(0), float(scale),
         int(max_seq_len), _ptr(alibi_slopes), qd, _kv_dtype(kv_cache_dtype, qd), float(kv_scale), _ptr(ws),
         ws.numel(), _stream()))
@@ -548,13 +565,15 @@ def evict_rows(
     _per_sequence(num_seqs, new_seq_lens, slot_mapping)
     _weights_of(weights, num_kv_heads, max_seq_len)
     _on_current_device(weights, key_cache, value_cache, seq_lens, new_seq_lens, slot_mapping)
+    _pointer_tables(key_cache, value_cache)
     if model_dtype not in (torch.float32, torch.bfloat16, torch.float16):
         raise _C.VtkvError(_C.EINVAL, f"unsupported model dtype {model_dtype}")
     lib = _C.lib()
     ws = _scratch(lib.vtkv_evict_rows_workspace_bytes(num_seqs, num_kv_heads, max_seq_len, keep_rows, recent_rows),
                   weights.device)
     _C.check(lib.vtkv_evict_rows(
-        _ptr(key_cache), _ptr(value_cache), _ptr(weights), weights.stride(0), weights.stride(1), weights.shape[0],
+        _ptr(key_cache), _ptr(value_cache), _ptr(weights), weights.stride(0), weights.stride(1),
+        _num_slots(weights, key_cache, value_cache),
         _ptr(slot_mapping), _ptr(seq_lens), _ptr(new_seq_lens), num_seqs, num_kv_heads, head_size,
         _kv_dtype(kv_cache_dtype, _DTYPES[model_dtype]), int(keep_rows), int(recent_rows), int(max_seq_len), _ptr(ws),
         ws.numel(), _stream()))

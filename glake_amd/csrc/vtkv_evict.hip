@@ -695,8 +695,9 @@ int vtkv_accumulate_attention_weights(float *weights, int64_t slot_stride, int64
   p.heads_wg = 1;
   while (p.heads_wg < waves && p.heads_wg < p.num_kv_heads) p.heads_wg *= 2;
   const int rows_wg = waves / p.heads_wg * kTileRows * kTiles;
-  const unsigned gx = (unsigned)((p.num_kv_heads + p.heads_wg - 1) / p.heads_wg * ((max_seq_len + rows_wg - 1) / rows_wg));
-  const unsigned sx = (unsigned)((max_seq_len + kSumRows - 1) / kSumRows);
+  const int64_t gx = (p.num_kv_heads + p.heads_wg - 1) / p.heads_wg * (((int64_t)max_seq_len + rows_wg - 1) / rows_wg);
+  VTKV_REQUIRE(gx * waves * 64 < (1ll << 31), "max_seq_len %d is too large", max_seq_len);
+  const unsigned sx = (unsigned)(((int64_t)max_seq_len + kSumRows - 1) / kSumRows);
   hipStream_t st = (hipStream_t)stream;
   const int step = (int)std::min<int64_t>(fit, 65535);
   for (int at = 0; at < num_seqs; at += step) {
@@ -706,7 +707,7 @@ int vtkv_accumulate_attention_weights(float *weights, int64_t slot_stride, int64
     p.seq_lens = seq_lens + at;
     p.logits = (float *)workspace;
     p.stats = p.logits + (int64_t)n * num_heads * p.pitch;
-    const dim3 grid(gx, 1, (unsigned)n);
+    const dim3 grid((unsigned)gx, 1, (unsigned)n);
     switch (head_size) {
       case 64: launch_logits<64>(p, kv, f16, grid, waves * 64, st); break;
       case 80: launch_logits<80>(p, kv, f16, grid, waves * 64, st); break;
@@ -733,7 +734,7 @@ int vtkv_evict_rows(const int64_t *k_ptrs, const int64_t *v_ptrs, float *weights
                     int recent_rows, int max_seq_len, void *workspace, int64_t workspace_bytes, void *stream) {
   VTKV_REQUIRE(k_ptrs && v_ptrs && weights && slot_ids && seq_lens && new_seq_lens, "null argument");
   VTKV_REQUIRE(num_seqs >= 0 && num_kv_heads > 0 && num_kv_heads <= 65535 && num_slots > 0, "bad sizes");
-  VTKV_REQUIRE((int64_t)num_seqs * num_kv_heads < 1 << 24, "too many sequences");
+  VTKV_REQUIRE((int64_t)num_seqs * num_kv_heads < (1 << 20), "too many sequences");
   VTKV_REQUIRE(vtkv::int4_head_size(head_size), "head_size %d is not supported (64, 80, 96, 112, 128, 256)", head_size);
   VTKV_REQUIRE(kv_dtype == VTKV_F32 || kv_dtype == VTKV_BF16 || kv_dtype == VTKV_F16 || kv_dtype == VTKV_FP8_E4M3 ||
                    kv_dtype == VTKV_INT4, "bad kv_dtype %d", kv_dtype);

@@ -245,6 +245,7 @@ def test_evict_moves_of_many_steps(env):
     evict_case(env, 21, [3000, 2101, 2500], 2100, 2000, 2, 128)
     evict_case(env, 22, [3000, 2101, 2500], 2100, 700, 2, 112, "int4")
     evict_case(env, 23, [17000, 16500], 8000, 500, 1, 64)  # (16384 old rows and a few more)
+    evict_case(env, 24, [16884, 9000], 8000, 500, 1, 64)  # (16384)
 
 
 def test_evict_negative_nan_stays(env):

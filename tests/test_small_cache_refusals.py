@@ -164,3 +164,21 @@ def test_python_refusals():
     for bad in (torch.zeros(2, 3, 8), torch.zeros(2, 2, 7), torch.zeros(2, 2, 8, dtype=torch.float64), torch.zeros(2, 2, 16)[..., ::2]):
         with pytest.raises(_C.VtkvError, match="weights"):
             ops._weights_of(bad, 2, 8)
+
+
+def test_pointer_tables():
+    ops._pointer_tables(0, 123)
+    for bad in (torch.zeros(4, dtype=torch.int64), torch.zeros(4, dtype=torch.int32)):
+        with pytest.raises(_C.VtkvError, match="pointer table"):
+            ops._pointer_tables(0, bad)
+    weights = torch.zeros(5, 2, 8)
+    assert ops._num_slots(weights, 0) == 5 and ops._num_slots(weights, torch.zeros(3, dtype=torch.int64), 0) == 3
+
+
+def test_cache_engine_refusals():
+    from glake_amd.worker.cache_engine import CacheEngine
+
+    for dtype, kind in ((torch.bfloat16, "int3"), (torch.bfloat16, "fp8"), (torch.uint8, "auto")):
+        with pytest.raises(_C.VtkvError):
+            CacheEngine(1, 2, 128, dtype, 1, 64, kv_cache_dtype=kind)
+    assert CacheEngine.get_cache_block_size(16, 8, 128, 2, torch.bfloat16, "int4") == 2 * 2 * 16 * 544

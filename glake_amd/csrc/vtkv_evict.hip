@@ -399,8 +399,8 @@ struct Unit<8> {
 // kHeldKeys old rows have their keys, and later the lists, in LDS; more are read again each time, their lists in the
 // workspace.  The first recent rows are asked for before the search starts.
 //   Bound by the bytes moved, each read and written once, and by the search before them (15 to 19 us when nothing moves).
-// 64 sequences of 8 kv heads of 128 bf16 elements that give up one row of 2049 and move 256 recent ones (134 MB read, as
-// many written): 38 us, 7.1 TB/s; 32 sequences of 3001 to 4096 rows cut to 2048, 512 of them recent: 84 us.  Four
+// 64 sequences of 8 kv heads of 128 bf16 elements that give up one row of 2049 and move 256 recent ones (139 MB read and
+// written): 38 us, 3.7 TB/s; 32 sequences of 3001 to 4096 rows cut to 2048, 512 of them recent: 84 us.  Four
 // pieces instead of two leave one workgroup per compute unit instead of two: 47 us and 85 us; without the second set of
 // pieces in flight 39 us and 109 us; keys and lists in memory instead of LDS: 39 us and 88 us.
 constexpr int kHeldKeys = 16384;

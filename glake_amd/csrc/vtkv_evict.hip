@@ -11,6 +11,7 @@
 #include "vtkv_attn_common.h"
 #include "vtkv_common.h"
 #include "vtkv_int4.h"
+#include "vtkv_int4_query.h"
 
 #include <algorithm>
 #include <cmath>
@@ -154,32 +155,14 @@ __global__ void __launch_bounds__(KV == 2 ? 512 : 256) attention_logits_kernel(W
     }
   }
   if constexpr (I4) {
-    float top = 0.f;
+    LargestQuery<F16> largest;
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s)
+    for (int s = 0; s < kSteps; ++s) largest.take(qop[s]);
+    const QueryScale q_scale = query_scale(largest.value());
+    q_back = p.scale_log2 * 0x1p24f * q_scale.down;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float x = unpack_16<F16>(qop[s][e >> 1], e & 1);
-        top = fmaxf(top, fabsf(x));
-        q_sum += x;
-      }
-    q_sum = sum_over_row_groups(q_sum) * p.scale_log2;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-    const int expo = min(max((int)(__builtin_bit_cast(unsigned, top) >> 23), 14), 254);
-    const float up = __builtin_bit_cast(float, (unsigned)(268 - expo) << 23);  // top * up in [2^14, 2^15)
-    q_back = p.scale_log2 * 0x1p24f / up;
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      float x[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = unpack_16<F16>(qop[s][e >> 1], e & 1) * up;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float f = r & 1 ? 0.0625f : 1.f;
-        qop[s][r] = pack_16x2<true>(x[r] * f, x[r + 4] * f);
-      }
-    }
+    for (int s = 0; s < kSteps; ++s) qop[s] = query_operand<F16>(qop[s], q_scale.up);
+    q_sum = query_sum(qop) * q_scale.down * p.scale_log2;
   }
   const float slope = p.alibi_slopes && h < hv ? p.alibi_slopes[h0 + h] * kLog2e : 0.f;
   const int row_at = 16 * (J == 2 ? j : 0) + 4 * g;  // this lane's rows of a tile: 16 J e + row_at + i

@@ -40,6 +40,7 @@
 #include "vtkv_attn_common.h"
 #include "vtkv_common.h"
 #include "vtkv_int4.h"
+#include "vtkv_int4_query.h"
 
 #include <algorithm>
 #include <cmath>
@@ -338,35 +339,17 @@ __global__ void __launch_bounds__(waves_of(D) * 64) int4_decode_kernel(DecodePar
     const int lane = opaque(tid & 63), g = lane >> 4, n = lane & 15, h = n % kHeads, word0 = word0_of(g);
     head = has_tile ? head_of_chunk(p, c.chunk, hs) : -1;
     len = len_of(c.b);
-    float top = 0.f, sum = 0.f;
+    LargestQuery<F16> largest;
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float x = unpack_16<F16>(raw[s][e >> 1], e & 1);
-        top = fmaxf(top, fabsf(x));
-        sum += x;
-      }
-    top = max_over_row_groups(top);
-#pragma unroll
-    for (int d = 1; d < 16; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-    sum = sum_over_row_groups(sum);
-    const int expo = min(max((int)(__builtin_bit_cast(unsigned, top) >> 23), 14), 254);
-    const float up = __builtin_bit_cast(float, (unsigned)(268 - expo) << 23);  // top * up in [2^14, 2^15)
-    const float q_back = (1.f / up) * 16777216.f * p.scale_log2;
-    q_sum = sum * p.scale_log2;
+    for (int s = 0; s < kSteps; ++s) largest.take(raw[s]);
+    const QueryScale q_scale = query_scale(largest.value());
+    const float q_back = q_scale.down * 16777216.f * p.scale_log2;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-      float x[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = unpack_16<F16>(raw[s][e >> 1], e & 1) * up;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float f = r & 1 ? 0.0625f : 1.f;
-        qop[s][r] = pack_16x2<true>(x[r] * f, x[r + 4] * f);
-      }
+      qop[s] = query_operand<F16>(raw[s], q_scale.up);
       __builtin_amdgcn_sched_barrier(0);
     }
+    q_sum = query_sum(qop) * q_scale.down * p.scale_log2;
     __builtin_amdgcn_sched_barrier(0);  // (what follows must not take registers from what precedes)
     slope = 0.f;
     if (p.alibi_slopes && head >= 0 && h < heads_of(p, head)) slope = p.alibi_slopes[first_head_of(p, head) + h] * kLog2e;

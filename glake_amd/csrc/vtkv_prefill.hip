@@ -40,6 +40,7 @@
 #include "vtkv_attn_common.h"
 #include "vtkv_common.h"
 #include "vtkv_int4.h"
+#include "vtkv_int4_query.h"
 
 #include <type_traits>
 
@@ -225,46 +226,25 @@ __global__ void __launch_bounds__(kThreads) prefill_attn_kernel(PrefillParams p)
   float sl = p.scale_log2;
   float q_sum[kNB];  // 4-bit rows: sum(q)
   if constexpr (I4) {
-    float top = 0.f;
+    LargestQuery<F16> largest;
 #pragma unroll
-    for (int nb = 0; nb < kNB; ++nb) {
-      q_sum[nb] = 0.f;
+    for (int nb = 0; nb < kNB; ++nb)
 #pragma unroll
-      for (int ks = 0; ks < kKS; ++ks)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float x = unpack_16<F16>(qop[nb][ks][e >> 1], e & 1);
-          top = fmaxf(top, fabsf(x));
-          q_sum[nb] += x;
-        }
-      q_sum[nb] = sum_over_row_groups(q_sum[nb]);
-    }
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+      for (int ks = 0; ks < kKS; ++ks) largest.take(qop[nb][ks]);
+    float top = largest.value();
     float *tops = reinterpret_cast<float *>(smem);
     if (lane == 0) tops[wave] = top;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) top = fmaxf(top, tops[w]);
     __syncthreads();
-    // the power of two that brings the workgroup's largest query value near 2^14 in fp16
-    const int expo = min(max((int)(__builtin_bit_cast(unsigned, top) >> 23), 14), 254);
-    const float up = __builtin_bit_cast(float, (unsigned)(268 - expo) << 23);
-    const float per_code = up * 0x1p-24f;  // a dot product with the codes over the one with the values 0..15
-    sl /= per_code;
+    const QueryScale q_scale = query_scale(top);
+    sl *= 0x1p24f * q_scale.down;
 #pragma unroll
     for (int nb = 0; nb < kNB; ++nb) {
 #pragma unroll
-      for (int ks = 0; ks < kKS; ++ks) {
-        float x[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = unpack_16<F16>(qop[nb][ks][e >> 1], e & 1) * up;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float f = r & 1 ? 0.0625f : 1.f;
-          qop[nb][ks][r] = pack_f16x2(x[r] * f, x[r + 4] * f);
-        }
-      }
+      for (int ks = 0; ks < kKS; ++ks) qop[nb][ks] = query_operand<F16>(qop[nb][ks], q_scale.up);
+      q_sum[nb] = query_sum(qop[nb]) * q_scale.down;
     }
   }
   // rows this wave needs: up to the limit of its last used column; its first column's limit says from

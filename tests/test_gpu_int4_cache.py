@@ -314,6 +314,31 @@ def test_decode_a_row_that_is_not_finite_stays_with_its_head(env):
         check(out[i, heads], want[heads], np.abs(v[i]).max(), 0.0, 2.0 ** -12)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+def test_a_query_that_is_not_finite_stays_with_its_head(env, dtype, value):
+    """Decode and prompt attention: the other heads of the same kv head and the other tokens are as without it."""
+    torch, ops = env
+    rng = np.random.default_rng(22)
+    lens, hq, hkv, d = [70, 90], 8, 2, 128
+    r, k, v = filled(rng, lens, hkv, d, [0, 1])
+    q, q_host = S.as_type(rng.standard_normal((2, hq, d)), dtypes(torch)[dtype])
+    q[1, 1, 5] = value
+    slots = torch.tensor([0, 1], device="cuda")
+    out = torch.empty(2, hq, d, dtype=torch.float32, device="cuda")
+    ops.paged_attention_v1(out, q, r.kp, r.vp, hkv, d ** -0.5, torch.tensor(lens, dtype=torch.int32, device="cuda"), 1, 90,
+                           None, "int4", 1.0, slots)
+    prompt = torch.empty(2, hq, d, dtype=torch.float32, device="cuda")
+    ops.prefill_attention(prompt, q, r.kp, r.vp, hkv, d ** -0.5, [1, 1], lens, slots, None, "int4")
+    for got, bound in ((out, 2.0 ** -12), (prompt, 2.0 ** -8)):  # (a unit with such a query is computed with bfloat16 values)
+        got = got.double().cpu().numpy()
+        assert np.isnan(got[1, 1]).all()
+        for i in range(2):
+            want = S.attention(q_host[i:i + 1], k[i], v[i], d ** -0.5)[0]
+            heads = [h for h in range(hq) if (i, h) != (1, 1)]
+            check(got[i, heads], want[heads], np.abs(v[i]).max(), 0.0, bound)
+
+
 def test_decode_in_a_graph_and_on_two_streams(env):
     torch, ops = env
     rng = np.random.default_rng(13)

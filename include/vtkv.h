@@ -447,7 +447,8 @@ int vtkv_decode_append_attention(void *out, const void *q, const void *key, cons
  *   seq_lens   device int32[num_seqs], at most max_seq_len (larger ones are cut off); 0 leaves the slot as it is
  *   slot_ids   device int64[num_seqs]; the slots of a call are distinct, a slot outside [0, num_slots) is skipped
  *   kv_dtype   q_dtype, VTKV_FP8_E4M3 with k_scale, or VTKV_INT4
- *   workspace  device scratch of vtkv_accumulate_attention_weights_workspace_bytes(...) bytes, any contents
+ *   workspace  device scratch of vtkv_accumulate_attention_weights_workspace_bytes(...) bytes, any contents, 16-byte
+ *              aligned; a smaller one serves as long as one sequence fits (the batch then runs in more parts)
  * Other arguments as for vtkv_decode_attention (q_dtype VTKV_BF16 or VTKV_F16).  Only K is read. */
 int64_t vtkv_accumulate_attention_weights_workspace_bytes(int num_seqs, int num_heads, int max_seq_len);
 int vtkv_accumulate_attention_weights(float *weights, int64_t slot_stride, int64_t head_stride, int64_t num_slots,

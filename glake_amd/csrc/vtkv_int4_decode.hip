@@ -9,7 +9,7 @@
 //  * K: two codes of a word masked in place (word & 0x000f000f, word & 0x00f000f0, the same of word >> 8) are the
 //    fp16 numbers c * 2^-24 and c * 2^-20 (denormals, which the fp16 MFMA takes as they are): five instructions for
 //    eight codes and no rounding.  The other factor 16 and the 2^24 go into q, which is brought to fp16 by a power of
-//    two per head (its largest value near 2^14): exact for bf16 and fp16 queries.
+//    two per query head (its largest value near 2^14; how exact that is: vtkv_int4_query.h).
 //  * V: the codes of 16 rows come out of LDS transposed (ds_read_b64_tr_b4: lane d of a group gets column d of 16
 //    rows) and are masked the same way: as bf16 numbers they are c * 2^-133 and c * 2^-129, in the denormals and the
 //    binade above them, where the bits count evenly.  p s comes with a factor of 2^60 (2^56 for the rows whose codes
@@ -327,8 +327,8 @@ __global__ void __launch_bounds__(waves_of(D) * 64) int4_decode_kernel(DecodePar
   };
 
   u32x4 qop[kSteps];
-  float q_sum, slope;  // logit = (s * q_back) * acc + z * q_sum [+ slope * distance]
-  float own_mul;       // what this lane multiplies its row's scale with: q_back (K), the power of two of P.V (V)
+  float q_back, q_sum, slope;  // logit = (s * 2^24 scale) * (acc * q_back) + z * q_sum [+ slope * distance]
+  float own_mul;               // what this lane multiplies its row's scale with: 2^24 scale (K), the power of two of P.V (V)
   int k_lane, v_lane, v_last, sz_lane, head = -1, len = 0;
   f32x4 acc[kDB];
   // a column's reference point, and how far a logit may be above it before it follows the maximum (-inf: no logit yet);
@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(waves_of(D) * 64) int4_decode_kernel(DecodePar
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) largest.take(raw[s]);
     const QueryScale q_scale = query_scale(largest.value());
-    const float q_back = q_scale.down * 16777216.f * p.scale_log2;
+    q_back = q_scale.down;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       qop[s] = query_operand<F16>(raw[s], q_scale.up);
@@ -370,7 +370,7 @@ __global__ void __launch_bounds__(waves_of(D) * 64) int4_decode_kernel(DecodePar
 #pragma unroll
     for (int d = 0; d < kDB; ++d) acc[d] = (f32x4){0.f, 0.f, 0.f, 0.f};
     // (this lane's row of the tile is 4 (lane & 7) + ..: its register of the P.V operands is odd where lane is)
-    own_mul = lane < 32 ? q_back : lane & 1 ? 0x1p56f : 0x1p60f;
+    own_mul = lane < 32 ? 0x1p24f * p.scale_log2 : lane & 1 ? 0x1p56f : 0x1p60f;
     m_ref = 0.f;
     lazy = -INFINITY;
     l_run = z_run = 0.f;
@@ -470,8 +470,8 @@ __global__ void __launch_bounds__(waves_of(D) * 64) int4_decode_kernel(DecodePar
 #pragma unroll
     for (int e = 0; e < kE; ++e)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) a[e][i] = J == 2 ? (j == 0 ? sa[0][i] : sa[1][i]) : sa[e][i];
-    auto logits = [&]() {
+      for (int i = 0; i < 4; ++i) a[e][i] = (J == 2 ? (j == 0 ? sa[0][i] : sa[1][i]) : sa[e][i]) * q_back;
+    {
 #pragma unroll
       for (int e = 0; e < kE; ++e)
 #pragma unroll
@@ -497,10 +497,10 @@ __global__ void __launch_bounds__(waves_of(D) * 64) int4_decode_kernel(DecodePar
       for (int e = 0; e < kE; ++e)
 #pragma unroll
         for (int i = 0; i < 4; ++i) top = fmaxf(top, x[e][i]);
-    };
-    logits();
+    }
     // The reference point of a column follows its maximum only when that has grown by more than 8 (a factor 256 in
-    // the weights): the rescale of the accumulators becomes rare.
+    // the weights): the rescale of the accumulators becomes rare.  (The logits follow by the same number, so that the
+    // largest is 0 exactly however large it was.)
     if (__builtin_amdgcn_ballot_w64(top > lazy) != 0) {
       const float t = max_over_row_groups(top);
       const bool moves = t > lazy;  // (its first logit, where lazy is -inf)
@@ -512,7 +512,11 @@ __global__ void __launch_bounds__(waves_of(D) * 64) int4_decode_kernel(DecodePar
       l_run *= alpha;
       z_run *= alpha;
       rescale(alpha);
-      logits();
+      const float up = moves ? t : 0.f;
+#pragma unroll
+      for (int e = 0; e < kE; ++e)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[e][i] -= up;
     }
     if constexpr (J == 1) {  // (twice the logits: registers are short until they are done)
       __builtin_amdgcn_sched_barrier(0);

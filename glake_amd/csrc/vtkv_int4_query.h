@@ -1,10 +1,12 @@
 // Queries on their way to the dot products with bare 4-bit codes (vtkv_int4.h), shared by the kernels that form them.
 //
 // The codes of a word come as fp16 numbers c * 2^-24 (registers 0 and 2 of an operand) and c * 2^-20 (1 and 3), register r
-// holding codes r and r + 4.  The other factor goes into q: one power of two brings the largest of the queries that share
-// an operand near 2^14 in fp16, the odd registers take a sixteenth of it.  Exact for bf16 and fp16 queries down to 2^-38 of the
-// largest.  The largest magnitude is found on pairs of 16-bit patterns and sum(q) comes from the matrix pipe: half the
-// instructions of the plain form and eight registers less in the decode kernel (its times are the same).
+// holding codes r and r + 4.  The other factor goes into q: a power of two per query head (and token) brings its largest value
+// near 2^14 in fp16, the odd registers take a sixteenth of it.  That is exact for a bf16 value down to 2^-27 of its head's
+// largest and for an fp16 value down to 2^-24; a smaller one is off by 2^-35 of the largest at most.  A head's dot products are
+// brought back by its own power, so what another head or token of the same operand holds does not touch them.  The largest
+// magnitude is found on pairs of 16-bit patterns and sum(q) comes from the matrix pipe: half the instructions of the plain
+// form and eight registers less in the decode kernel (its times are the same).
 #pragma once
 #include "vtkv_attn_common.h"
 
@@ -27,18 +29,10 @@ struct LargestQuery {
       most = __builtin_elementwise_max(most, __builtin_bit_cast(i16x2, raised));
     }
   }
-  // over the lanes of the wave
+  // of the lane's column, whose values its four row groups hold
   __device__ __forceinline__ float value() const {
     const unsigned bits = (unsigned)max((int)most[0], (int)most[1]) - kStep;
-    float x = unpack_16<F16>(bits, 0);
-#define VTKV_JOIN(CTRL) \
-  x = fmaxf(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true)))
-    VTKV_JOIN(0xb1);   // lanes 1 0 3 2 of each four
-    VTKV_JOIN(0x4e);   // 2 3 0 1
-    VTKV_JOIN(0x141);  // each eight mirrored
-    VTKV_JOIN(0x140);  // each sixteen mirrored
-#undef VTKV_JOIN
-    return max_over_row_groups(x);
+    return max_over_row_groups(unpack_16<F16>(bits, 0));
   }
 };
 

@@ -59,3 +59,54 @@ def test_decode_weights_are_not_cut_off(env, hq, d):
     ops.paged_attention_v1(out, q, r.kp, r.vp, 1, -np.log(p), i32([n]), 1, n, None, "int4", 1.0, i64([0]))
     err = np.abs(out.double().cpu().numpy() / 15.0 - 1.0)
     assert err.max() <= 2.5 * 2.0 ** -18, f"{err.max() * 2.0 ** 18:.2f} * 2^-18"
+
+
+# ------------------------------------------------------------------------------------------------ queries far apart
+def filled(rng, lens, hkv, d, k_factor=1.0, v_factor=1.0):
+    """Ranges with lens[i] rows of sequence i in slot i, and the rows' values."""
+    r = S.Ranges(len(lens), max(lens), S.row_bytes(hkv, d))
+    k, v = [], []
+    for i, n in enumerate(lens):
+        for values, cache, f in ((k, r.k, k_factor), (v, r.v, v_factor)):
+            x = S.quantise(S.to_bf16(f * S.model_values(rng, (n, hkv, d))))
+            values.append(S.values(*x))
+            put(cache, i, *x)
+    return r, k, v
+
+
+@pytest.mark.parametrize("value", [2.0 ** 26, 1e30])
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (16, 1, 80), (8, 8, 64)])
+def test_a_large_query_stays_with_its_head(env, value, hq, hkv, d):
+    """One large finite number in one head of one token: decode, prompts and weights are, everywhere else, as they are
+    without it, and that head attends to the one row that is largest there.  Tolerances as for ordinary values: 2^-12 of the
+    largest value (decode), 2^-10 + 2^-11 (prompts), 2^-12 of a weight (a sum over the heads of a kv head)."""
+    torch, ops = env
+    rng = np.random.default_rng(40)
+    lens, query_lens = [70, 90], [40, 33]
+    r, k, v = filled(rng, lens, hkv, d)
+    scale, slots = d ** -0.5, i64([0, 1])
+    v_max = [np.abs(x).max() for x in v]
+
+    x = rng.standard_normal((2, hq, d))
+    x[1, 1, 5] = value
+    q, qh = S.as_type(x, torch.bfloat16)
+    out = torch.empty(2, hq, d, device="cuda")
+    ops.paged_attention_v1(out, q, r.kp, r.vp, hkv, scale, i32(lens), 1, 90, None, "int4", 1.0, slots)
+    weights = torch.zeros(2, hkv, 90, device="cuda")
+    ops.accumulate_attention_weights(weights, q, r.kp, hkv, scale, i32(lens), 90, slots, None, "int4")
+    for i, n in enumerate(lens):
+        want = S.attention(qh[i:i + 1], k[i], v[i], scale)[0]
+        assert (np.abs(out[i].double().cpu().numpy() - want) <= 2.0 ** -12 * v_max[i]).all()
+        p = S.softmax(qh[i:i + 1], k[i], scale)[0].reshape(hkv, hq // hkv, n).sum(1)
+        assert (np.abs(weights[i, :, :n].double().cpu().numpy() - p) <= 2.0 ** -12 * p + 1e-30).all()
+
+    x = rng.standard_normal((sum(query_lens), hq, d))
+    x[query_lens[0] + 9, 1, 5] = value
+    q, qh = S.as_type(x, torch.bfloat16)
+    out = torch.empty(q.shape, device="cuda")
+    ops.prefill_attention(out, q, r.kp, r.vp, hkv, scale, query_lens, lens, slots, None, "int4")
+    at = 0
+    for i, n in enumerate(query_lens):
+        want = S.attention(qh[at:at + n], k[i], v[i], scale, np.arange(lens[i] - n, lens[i]) + 1)
+        assert (np.abs(out[at:at + n].double().cpu().numpy() - want) <= (2.0 ** -10 + 2.0 ** -11) * v_max[i]).all()
+        at += n

@@ -13,8 +13,10 @@
 //  * V: the codes of 16 rows come out of LDS transposed (ds_read_b64_tr_b4: lane d of a group gets column d of 16
 //    rows) and are masked the same way: as bf16 numbers they are c * 2^-133 and c * 2^-129, in the denormals and the
 //    binade above them, where the bits count evenly.  p s comes with a factor of 2^60 (2^56 for the rows whose codes
-//    stand 2^4 higher) and is carried as a bf16 head and a bf16 tail (2^-18 relative, rounded).  Scales up to 2^60
-//    fit; what p s is below 2^-57 loses bits (an absolute error below 2^-53).
+//    stand 2^4 higher) and is carried as a bf16 head and a bf16 tail (2^-18 relative, rounded).  What p s is below 2^-57
+//    loses bits (values of 1e-18 still come out within 1e-5 of their size, values of 1e-22 within 1e-2).  Scales of 2^60
+//    and more, whose p s may leave the fp32 range, make the result of their query head NaN or infinite; the second kernel
+//    computes such a result again, plainly (plain_attention).
 //
 // How it moves data.  HBM-bound: 2 rows of 68 bytes per token and kv head (head size 128).  A workgroup takes whole
 // rows (or eight kv heads of them): a stage of 64 rows (512 / kv heads when there are fewer than eight) of K and V goes
@@ -712,8 +714,75 @@ __global__ void __launch_bounds__(waves_of(D) * 64) int4_decode_kernel(DecodePar
   }
 }
 
+// Attention of one query head over the values themselves, in fp32 on the vector unit by a workgroup of 256 threads: for
+// results that the kernel above could not hold (and for those that are not finite whichever way they are computed).  A thread
+// takes whole rows for their logits, then, 256 rows at a time, a dim for the sum of the values, whose weights are normalised
+// first: it stays as small as the values are.
+template <int D, bool F16>
+__device__ void plain_attention(const DecodeParams &p, int b, int head, int len) {
+  __shared__ float s_q[D], s_p[256], s_top[256];
+  const int tid = threadIdx.x, real = head / p.group_real, kv_real = p.num_kv_heads / p.kv_split;
+  const int64_t slot = p.slot_ids[b];
+  const char *const k_rows = (const char *)(uintptr_t)p.k_ptrs[slot], *const v_rows = (const char *)(uintptr_t)p.v_ptrs[slot];
+  const int codes_at = real * (D / 2), pair_at = kv_real * (D / 2) + 4 * real;
+  const float slope = p.alibi_slopes ? p.alibi_slopes[head] * kLog2e : 0.f;
+  if (tid < D) s_q[tid] = unpack_16<F16>(p.q[(int64_t)b * p.q_stride + (int64_t)head * D + tid], 0) * p.scale_log2;
+  __syncthreads();
+  auto logit = [&](int r) {
+    const char *row = k_rows + (int64_t)r * p.row_bytes;
+    const unsigned *codes = reinterpret_cast<const unsigned *>(row + codes_at);
+    const unsigned pair = *reinterpret_cast<const unsigned *>(row + pair_at);
+    const float s = __builtin_bit_cast(float, pair << 16), z = __builtin_bit_cast(float, pair & 0xffff0000u);
+    float x = 0.f;
+#pragma unroll 1
+    for (int w = 0; w < D / 8; ++w)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        x = __builtin_fmaf(s_q[8 * w + i], __builtin_fmaf((float)(codes[w] >> (4 * i) & 15u), s, z), x);
+    return __builtin_fmaf(slope, (float)(r - len + 1), x);
+  };
+  // ---- maximum and sum
+  float m = -INFINITY, l = 0.f;
+#pragma unroll 1
+  for (int r = tid; r < len; r += 256) {
+    const float x = logit(r), top = fmaxf(m, x);
+    l = l * (m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top)) + __builtin_amdgcn_exp2f(x - top);
+    m = top;
+  }
+  s_top[tid] = m;
+  __syncthreads();
+  float all = -INFINITY;
+  for (int i = 0; i < 256; ++i) all = fmaxf(all, s_top[i]);
+  s_p[tid] = m == -INFINITY ? l : l * __builtin_amdgcn_exp2f(m - all);
+  __syncthreads();
+  float sum = 0.f;
+  for (int i = 0; i < 256; ++i) sum += s_p[i];
+  const float inv = 1.f / sum;
+  // ---- the values
+  float o = 0.f;
+#pragma unroll 1
+  for (int r0 = 0; r0 < len; r0 += 256) {
+    __syncthreads();
+    if (r0 + tid < len) s_p[tid] = __builtin_amdgcn_exp2f(logit(r0 + tid) - all) * inv;
+    __syncthreads();
+    if (tid < D) {
+      const char *row = v_rows + (int64_t)r0 * p.row_bytes;
+#pragma unroll 1
+      for (int i = 0; i < min(256, len - r0); ++i, row += p.row_bytes) {
+        const unsigned pair = *reinterpret_cast<const unsigned *>(row + pair_at), code = (unsigned char)row[codes_at + tid / 2] >> (4 * (tid & 1)) & 15u;
+        o = __builtin_fmaf(s_p[i], __builtin_fmaf((float)code, __builtin_bit_cast(float, pair << 16), __builtin_bit_cast(float, pair & 0xffff0000u)), o);
+      }
+    }
+  }
+  if (tid < D) {
+    const int64_t at = ((int64_t)b * p.num_heads + head) * D + tid;
+    if (p.out_f32) reinterpret_cast<float *>(p.out)[at] = o;
+    else reinterpret_cast<uint16_t *>(p.out)[at] = f32_to_16<F16>(o);
+  }
+}
+
 // Merges the partial results of a (sequence, query head); writes zeros where there are no rows.  The partial results are
-// dealt to groups of D / 4 lanes with four values each.
+// dealt to groups of D / 4 lanes with four values each.  A result that is not finite is computed again.
 template <int D, bool F16>
 __global__ void __launch_bounds__(256) int4_merge_kernel(DecodeParams p) {
   constexpr int kLanes = D / 4, kGroups = 256 / kLanes, kUnroll = 4;
@@ -730,7 +799,16 @@ __global__ void __launch_bounds__(256) int4_merge_kernel(DecodeParams p) {
   const int len = min(p.seq_lens[b], p.max_seq_len);
   const int32_t *span = p.spans + 2 * ((int64_t)b * p.chunks + chunk);
   const int first = len > 0 ? span[0] : 0, i0 = first / 2, i1 = len > 0 ? span[1] : -1;
-  if (i0 == i1) return;
+  if (i0 == i1) {  // one span held all rows and has written the result
+    bool lost = false;
+    if (threadIdx.x < D) {
+      const int64_t at = ((int64_t)b * p.num_heads + head) * D + threadIdx.x;
+      if (p.out_f32) lost = (reinterpret_cast<const unsigned *>(p.out)[at] & 0x7f800000u) == 0x7f800000u;
+      else lost = (~reinterpret_cast<const uint16_t *>(p.out)[at] & (F16 ? 0x7c00u : 0x7f80u)) == 0;
+    }
+    if (__syncthreads_or(lost)) plain_attention<D, F16>(p, b, head, len);
+    return;
+  }
   const int grp = threadIdx.x / kLanes, d = threadIdx.x % kLanes * 4;
   float m = -INFINITY, l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
@@ -768,6 +846,7 @@ __global__ void __launch_bounds__(256) int4_merge_kernel(DecodeParams p) {
     }
   }
   __syncthreads();
+  bool lost = false;
   if (threadIdx.x < D) {
     float mm = -INFINITY, ll = 0.f, oo = 0.f;
     for (int k = 0; k < kGroups; ++k) mm = fmaxf(mm, s_m[k]);
@@ -780,7 +859,9 @@ __global__ void __launch_bounds__(256) int4_merge_kernel(DecodeParams p) {
     const int64_t at = ((int64_t)b * p.num_heads + head) * D + threadIdx.x;
     if (p.out_f32) reinterpret_cast<float *>(p.out)[at] = r;
     else reinterpret_cast<uint16_t *>(p.out)[at] = f32_to_16<F16>(r);
+    lost = (__builtin_bit_cast(unsigned, r) & 0x7f800000u) == 0x7f800000u;
   }
+  if (__syncthreads_or(lost)) plain_attention<D, F16>(p, b, head, len);
 }
 
 template <int D>

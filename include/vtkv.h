@@ -333,7 +333,9 @@ int64_t vtkv_decode_attention_workspace_bytes(int num_seqs, int num_heads, int h
  * kv_dtype VTKV_INT4 (bf16 and fp16 queries, every head size and head count): a kernel of its own over 4-bit rows
  * (see vtkv_kv_row_bytes), also through vtkv_decode_attention_noalloc and vtkv_prefill_attention, not through
  * vtkv_decode_attention_v2 and vtkv_decode_append_attention; partition_tokens, k_scale and v_scale are not used, and a
- * sequence of length 0 (a padded batch) gets zeros. */
+ * sequence of length 0 (a padded batch) gets zeros.  Cached values of any finite size are served; a query head whose V rows
+ * have scales of 2^60 and more, or whose result is not finite, is computed a second time, plainly and much more slowly.  V
+ * values below 1e-18 lose bits (1e-22: about 1 % of the largest). */
 int vtkv_decode_attention(void *out, const void *q, const int64_t *k_ptrs, const int64_t *v_ptrs,
                           const int64_t *slot_ids, const int32_t *seq_lens, int num_seqs, int num_heads,
                           int num_kv_heads, int head_size, int64_t q_stride, float scale, int max_seq_len,
@@ -406,7 +408,8 @@ int vtkv_prefill_unit_tokens(int num_heads, int num_kv_heads, int kv_dtype);
  * or 256 (the kernel is tuned for 128; units hold vtkv_prefill_unit_tokens_for(...) tokens), q_dtype
  * VTKV_BF16 or VTKV_F16, kv_dtype = q_dtype or VTKV_FP8_E4M3 with k_scale / v_scale, out_dtype = q_dtype or
  * VTKV_F32; the longest-units-first order inside each sequence, sequence by sequence, lets every row be fetched
- * from HBM once.  q_dtype VTKV_F32 with kv_dtype = out_dtype = VTKV_F32 (float32 models): every token attends
+ * from HBM once.  Values of V are carried in fp16 (below 2^-14 they lose bits, below 2^-25 they vanish); a unit that meets
+ * larger ones than fp16 holds is computed again with them in bf16.  q_dtype VTKV_F32 with kv_dtype = out_dtype = VTKV_F32 (float32 models): every token attends
  * through the float32 decode kernel by itself, without reuse of rows between tokens. */
 int vtkv_prefill_attention(void *out, const void *q, const int64_t *k_ptrs, const int64_t *v_ptrs,
                            const int64_t *slot_ids, const int32_t *units, int num_units, int num_heads,

@@ -110,3 +110,88 @@ def test_a_large_query_stays_with_its_head(env, value, hq, hkv, d):
         want = S.attention(qh[at:at + n], k[i], v[i], scale, np.arange(lens[i] - n, lens[i]) + 1)
         assert (np.abs(out[at:at + n].double().cpu().numpy() - want) <= (2.0 ** -10 + 2.0 ** -11) * v_max[i]).all()
         at += n
+
+
+# ------------------------------------------------------------------------------------------------ large and small numbers
+def attend(ops, r, q, hkv, lens, out_dtype=None):
+    import torch
+
+    b, hq, d = q.shape
+    out = torch.full(q.shape, 55.0, dtype=out_dtype or torch.float32, device="cuda")
+    ops.paged_attention_v1(out, q, r.kp, r.vp, hkv, d ** -0.5, i32(lens), 1, max(lens), None, "int4", 1.0, i64(list(range(b))))
+    return out
+
+
+@pytest.mark.parametrize("lens", [[200, 33], [9001]])
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (16, 1, 80), (8, 8, 256)])
+@pytest.mark.parametrize("factor", [1e18, 1e20, 1e30, 1e37])
+def test_decode_of_large_finite_values(env, lens, hq, hkv, d, factor):
+    """Results of spans that hold a whole sequence (200, 33 rows) and of several spans (9001).  The tolerance of ordinary
+    values, relative to the largest value."""
+    torch, ops = env
+    rng = np.random.default_rng(41)
+    r, k, v = filled(rng, lens, hkv, d, v_factor=factor)
+    q, qh = S.as_type(rng.standard_normal((len(lens), hq, d)), torch.bfloat16)
+    got, rounded = attend(ops, r, q, hkv, lens), attend(ops, r, q, hkv, lens, torch.bfloat16)
+    for i in range(len(lens)):
+        want = S.attention(qh[i:i + 1], k[i], v[i], d ** -0.5)[0]
+        assert (np.abs(got[i].double().cpu().numpy() - want) <= 2.0 ** -12 * np.abs(v[i]).max()).all()
+    assert torch.equal(got.bfloat16(), rounded)
+
+
+@pytest.mark.parametrize("n", [100, 7000])
+def test_decode_of_one_large_row_without_weight(env, n):
+    """A row of 1e25 that no query pays anything to (2^-200), among ordinary ones: the result is theirs."""
+    torch, ops = env
+    rng = np.random.default_rng(42)
+    hq, hkv, d, at = 8, 2, 128, 77
+    r, k, v = filled(rng, [n], hkv, d)
+    k[0][at], v[0][at] = 0.0, 0.0
+    big = S.quantise(S.to_bf16(1e25 * rng.standard_normal((1, hkv, d))))
+    r.v[0, at] = torch.from_numpy(S.pack(*big)).cuda()[0]
+    low = S.quantise(np.full((1, hkv, d), -1600.0))  # (queries are positive: far below every other row)
+    r.k[0, at] = torch.from_numpy(S.pack(*low)).cuda()[0]
+    q, qh = S.as_type(np.abs(rng.standard_normal((1, hq, d))) * 0.2, torch.bfloat16)
+    k[0][at] = -1600.0
+    got = attend(ops, r, q, hkv, [n])
+    want = S.attention(qh, k[0], v[0], d ** -0.5)[0]
+    assert (np.abs(got[0].double().cpu().numpy() - want) <= 2.0 ** -12 * np.abs(v[0]).max()).all()
+
+
+@pytest.mark.parametrize("factor", [1e30, 1e-30])
+def test_large_keys_of_small_queries_and_the_other_way_round(env, factor):
+    """Keys and queries whose products are ordinary numbers: decode, prompt and weights as for ordinary ones."""
+    torch, ops = env
+    rng = np.random.default_rng(43)
+    lens, hq, hkv, d = [300, 90], 8, 2, 128
+    r, k, v = filled(rng, lens, hkv, d, k_factor=factor)
+    q, qh = S.as_type(rng.standard_normal((sum(lens), hq, d)) / factor, torch.bfloat16)
+    out = torch.empty(q.shape, device="cuda")
+    ops.prefill_attention(out, q, r.kp, r.vp, hkv, d ** -0.5, lens, lens, i64([0, 1]), None, "int4")
+    ends = [lens[0] - 1, sum(lens) - 1]
+    last = attend(ops, r, q[ends], hkv, lens)
+    weights = torch.zeros(2, hkv, 300, device="cuda")
+    ops.accumulate_attention_weights(weights, q[ends], r.kp, hkv, d ** -0.5, i32(lens), 300, i64([0, 1]), None, "int4")
+    at = 0
+    for i, n in enumerate(lens):
+        want = S.attention(qh[at:at + n], k[i], v[i], d ** -0.5, np.arange(n) + 1)
+        top = np.abs(v[i]).max()
+        assert (np.abs(out[at:at + n].double().cpu().numpy() - want) <= (2.0 ** -10 + 2.0 ** -11) * top).all()
+        assert (np.abs(last[i].double().cpu().numpy() - want[-1]) <= 2.0 ** -12 * top).all()
+        p = S.softmax(qh[ends[i]:ends[i] + 1], k[i], d ** -0.5)[0].reshape(hkv, hq // hkv, n).sum(1)
+        assert (np.abs(weights[i, :, :n].double().cpu().numpy() - p) <= 2.0 ** -12 * p).all()
+        at += n
+
+
+@pytest.mark.parametrize("factor", [1e-6, 1e-9, 1e-15, 1e-18])
+def test_decode_of_small_values(env, factor):
+    """Down to 1e-18 values keep the relative tolerance of ordinary ones."""
+    torch, ops = env
+    rng = np.random.default_rng(44)
+    lens, hq, hkv, d = [200, 1033], 8, 2, 128
+    r, k, v = filled(rng, lens, hkv, d, v_factor=factor)
+    q, qh = S.as_type(rng.standard_normal((2, hq, d)) * 1.5, torch.bfloat16)
+    got = attend(ops, r, q, hkv, lens)
+    for i in range(2):
+        want = S.attention(qh[i:i + 1], k[i], v[i], d ** -0.5)[0]
+        assert (np.abs(got[i].double().cpu().numpy() - want) <= 2.0 ** -12 * np.abs(v[i]).max()).all()

@@ -400,8 +400,9 @@ __global__ void __launch_bounds__(kEvictThreads, 8) evict_kernel(EvictParams p) 
   const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63;
   const int n = min(p.seq_lens[seq], p.max_seq_len);
   const int64_t slot = p.slot_ids[seq];
-  if (kvh == 0 && tid == 0 && p.new_seq_lens != p.seq_lens) p.new_seq_lens[seq] = max(0, min(n, p.keep));
-  if (n <= p.keep || slot < 0 || slot >= p.num_slots) return;
+  const bool skipped = slot < 0 || slot >= p.num_slots;  // (its rows stay where they are, and so does its length)
+  if (kvh == 0 && tid == 0 && p.new_seq_lens != p.seq_lens) p.new_seq_lens[seq] = skipped ? p.seq_lens[seq] : max(0, min(n, p.keep));
+  if (n <= p.keep || skipped) return;
   const int heavy = p.keep - p.recent, old = n - p.recent;  // old > heavy >= 0
   float *w = p.weights + slot * p.slot_stride + kvh * p.head_stride;
   const bool held = p.held;
@@ -614,9 +615,9 @@ __global__ void __launch_bounds__(kEvictThreads, 8) evict_kernel(EvictParams p) 
 }
 
 // The new lengths where they replace the old ones (which every workgroup of the kernel above reads).
-__global__ void __launch_bounds__(256) cut_lengths_kernel(int32_t *lens, int num_seqs, int keep) {
+__global__ void __launch_bounds__(256) cut_lengths_kernel(int32_t *lens, const int64_t *slot_ids, int64_t num_slots, int num_seqs, int keep) {
   const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i < num_seqs) lens[i] = max(0, min(lens[i], keep));
+  if (i < num_seqs && slot_ids[i] >= 0 && slot_ids[i] < num_slots) lens[i] = max(0, min(lens[i], keep));
 }
 
 }  // namespace
@@ -758,7 +759,8 @@ int vtkv_evict_rows(const int64_t *k_ptrs, const int64_t *v_ptrs, float *weights
   else
     hipLaunchKernelGGL(evict_kernel<8>, grid, dim3(kEvictThreads), lds, st, p);
   if (new_seq_lens == seq_lens)
-    hipLaunchKernelGGL(cut_lengths_kernel, dim3((unsigned)((num_seqs + 255) / 256)), dim3(256), 0, st, new_seq_lens, num_seqs, keep_rows);
+    hipLaunchKernelGGL(cut_lengths_kernel, dim3((unsigned)((num_seqs + 255) / 256)), dim3(256), 0, st, new_seq_lens, slot_ids,
+                       num_slots, num_seqs, keep_rows);
   VTKV_HIP(hipGetLastError());
   return VTKV_OK;
 }

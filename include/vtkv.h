@@ -468,7 +468,8 @@ int vtkv_accumulate_attention_weights(float *weights, int64_t slot_stride, int64
  * evicted ones below heavy; the recent rows move to [heavy, keep_rows) in order.  weights moves with the rows and is
  * zero in [keep_rows, n).  new_seq_lens[b] = min(seq_lens[b], keep_rows) (may be seq_lens itself).  Rows in [keep_rows, n)
  * of the ranges are left as they were.
- *   seq_lens   device int32[num_seqs], at most max_seq_len; slots are distinct, one outside [0, num_slots) is skipped
+ *   seq_lens   device int32[num_seqs], at most max_seq_len; slots are distinct, a sequence whose slot lies outside
+ *              [0, num_slots) is skipped: its new length is its old one
  *   kv_dtype   the rows' type: VTKV_F32, VTKV_BF16, VTKV_F16, VTKV_FP8_E4M3 or VTKV_INT4
  *   workspace  device scratch of vtkv_evict_rows_workspace_bytes(...) bytes, any contents, 16-byte aligned
  * The rows of a head are no longer in the order of their tokens afterwards (attention without ALiBi does not mind).  The

@@ -195,3 +195,25 @@ def test_decode_of_small_values(env, factor):
     for i in range(2):
         want = S.attention(qh[i:i + 1], k[i], v[i], d ** -0.5)[0]
         assert (np.abs(got[i].double().cpu().numpy() - want) <= 2.0 ** -12 * np.abs(v[i]).max()).all()
+
+
+# ------------------------------------------------------------------------------------------------ slots
+@pytest.mark.parametrize("alias", [False, True])
+@pytest.mark.parametrize("kind", ["auto", "int4"])
+def test_evict_leaves_sequences_of_foreign_slots_alone(env, kind, alias):
+    """Slots outside the weights (slot 3 has ranges but no weights) and outside everything: rows, weights and lengths stay."""
+    torch, ops = env
+    rng = np.random.default_rng(50)
+    hkv, d, keep, recent, lens, slots = 2, 64, 40, 10, [90, 60, 100, 30, 75], [1, 3, -1, 1 << 40, 0]
+    r = S.Ranges(4, 100, S.row_bytes(hkv, d) if kind == "int4" else hkv * d * 2)
+    for t in (r.k, r.v):
+        t.copy_(torch.from_numpy(rng.integers(0, 256, t.shape, dtype=np.uint8)).cuda())
+    w = torch.rand(2, hkv, 100, device="cuda")
+    before = [x.clone() for x in (r.k, r.v, w)]
+    lens_t = i32(lens)
+    new = lens_t if alias else torch.full_like(lens_t, -7)
+    ops.evict_rows(r.kp, r.vp, w, lens_t, new, keep, recent, 100, i64(slots), hkv, d, kind)
+    assert new.tolist() == [40, 60, 100, 30, 40]
+    for a, b in zip((r.k, r.v), before):
+        assert torch.equal(a[2:], b[2:]) and not torch.equal(a[0, :40], b[0, :40]) and not torch.equal(a[1, :40], b[1, :40])
+    assert (w[1, :, 40:90] == 0).all() and (w[0, :, 40:75] == 0).all() and torch.equal(w[:, :, 90:], before[2][:, :, 90:])

@@ -173,6 +173,7 @@ __global__ void __launch_bounds__(waves_of(D) * 64) int4_decode_kernel(DecodePar
     int local[kPer], sum = 0;
     const bool in_table = tid < min(B, kPtrTable);
     const int64_t slot = in_table ? p.slot_ids[tid] : 0;
+    const int own_len = in_table ? min(p.seq_lens[tid], p.max_seq_len) : 0;
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
       const int idx = tid * kPer + k;
@@ -182,10 +183,10 @@ __global__ void __launch_bounds__(waves_of(D) * 64) int4_decode_kernel(DecodePar
         if (rows > 0) sum += (rows - 1) / kUnitRows + 1 + p.part_units;
       }
     }
-    if (in_table) {
+    if (in_table) reinterpret_cast<int *>(s_ptr + 2 * kPtrTable)[tid] = own_len;
+    if (own_len > 0) {  // (the slot of a sequence without rows is not followed: a padded entry may hold anything)
       s_ptr[2 * tid] = (uint64_t)p.k_ptrs[slot];
       s_ptr[2 * tid + 1] = (uint64_t)p.v_ptrs[slot];
-      reinterpret_cast<int *>(s_ptr + 2 * kPtrTable)[tid] = min(p.seq_lens[tid], p.max_seq_len);
     }
     int incl = sum;
 #pragma unroll

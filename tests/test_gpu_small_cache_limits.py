@@ -217,3 +217,39 @@ def test_evict_leaves_sequences_of_foreign_slots_alone(env, kind, alias):
     for a, b in zip((r.k, r.v), before):
         assert torch.equal(a[2:], b[2:]) and not torch.equal(a[0, :40], b[0, :40]) and not torch.equal(a[1, :40], b[1, :40])
     assert (w[1, :, 40:90] == 0).all() and (w[0, :, 40:75] == 0).all() and torch.equal(w[:, :, 90:], before[2][:, :, 90:])
+
+
+def test_empty_sequences_may_have_any_slot(env):
+    """Padded entries (length 0) whose slots lie in no table, below and above 256 sequences: zeros, and nobody else notices;
+    a step's write skips them by their byte offset, the weights by their length."""
+    torch, ops = env
+    rng = np.random.default_rng(51)
+    hq, hkv, d, b = 8, 2, 128, 300
+    lens = [0] * b
+    for i, n in ((0, 40), (7, 1), (255, 90), (256, 33), (299, 5)):
+        lens[i] = n
+    held = [n for n in lens if n]
+    r, k, v = filled(rng, held, hkv, d)
+    slots, at = [], 0
+    for i, n in enumerate(lens):
+        slots.append(at if n else [-1, 1 << 40, -(1 << 40)][i % 3])
+        at += n > 0
+    q, qh = S.as_type(rng.standard_normal((b, hq, d)), torch.bfloat16)
+    out = torch.full((b, hq, d), 55.0, device="cuda")
+    ops.paged_attention_v1(out, q, r.kp, r.vp, hkv, d ** -0.5, i32(lens), 1, 100, None, "int4", 1.0, i64(slots))
+    weights = torch.zeros(len(held), hkv, 100, device="cuda")
+    ops.accumulate_attention_weights(weights, q, r.kp, hkv, d ** -0.5, i32(lens), 100, i64(slots), None, "int4")
+    at = 0
+    for i, n in enumerate(lens):
+        if not n:
+            assert (out[i] == 0).all()
+            continue
+        want = S.attention(qh[i:i + 1], k[at], v[at], d ** -0.5)[0]
+        assert (np.abs(out[i].double().cpu().numpy() - want) <= 2.0 ** -12 * np.abs(v[at]).max()).all()
+        p = S.softmax(qh[i:i + 1], k[at], d ** -0.5)[0].reshape(hkv, hq // hkv, n).sum(1)
+        assert (np.abs(weights[at, :, :n].double().cpu().numpy() - p) <= 2.0 ** -12 * p).all() and (weights[at, :, n:] == 0).all()
+        at += 1
+    key = torch.zeros(b, hkv, d, dtype=torch.bfloat16, device="cuda")
+    before = r.k.clone()
+    ops.reshape_and_cache(key, key, r.kp, r.vp, i64([-1] * b), i64([-1] * b), None, None, 1, hkv, d, "int4")
+    assert torch.equal(r.k, before)

@@ -335,6 +335,16 @@ void launch_logits(const WeightParams &p, int kv, bool f16, dim3 grid, int threa
     launch_logits<D, 1>(p, kv, f16, grid, threads, st);
 }
 
+// No two (slot, kv head) of the weights share one of their `rows` first elements (an expanded tensor's would: workgroups
+// would add to them, or move them, at the same time).
+bool weights_apart(int64_t slot_stride, int64_t head_stride, int64_t num_slots, int num_kv_heads, int rows) {
+  typedef __int128 wide;
+  if (num_kv_heads > 1 && head_stride < rows) return false;
+  if (num_slots > 1 && slot_stride < rows) return false;
+  return num_kv_heads == 1 || num_slots == 1 || slot_stride >= (wide)(num_kv_heads - 1) * head_stride + rows ||
+         head_stride >= (wide)(num_slots - 1) * slot_stride + rows;
+}
+
 int64_t weight_pitch(int max_seq_len) { return ((int64_t)max_seq_len + kTileRows - 1) / kTileRows * kTileRows; }
 int64_t weight_bytes_per_seq(int num_heads, int max_seq_len) {
   const int64_t pitch = weight_pitch(max_seq_len);
@@ -647,6 +657,8 @@ int vtkv_accumulate_attention_weights(float *weights, int64_t slot_stride, int64
   VTKV_REQUIRE(q_stride >= (int64_t)num_heads * head_size && q_stride % 8 == 0 && (uintptr_t)q % 16 == 0,
                "q rows must be 16-byte aligned and at least num_heads*head_size apart");
   VTKV_REQUIRE(max_seq_len > 0 && num_slots > 0, "max_seq_len and num_slots must be > 0");
+  VTKV_REQUIRE(weights_apart(slot_stride, head_stride, num_slots, num_kv_heads, max_seq_len),
+               "weights of different slots and kv heads overlap");
   VTKV_REQUIRE(num_heads <= 65535, "too many query heads");
   VTKV_REQUIRE(vtkv_kv_row_bytes(num_kv_heads, head_size, kv_dtype) < (4 << 20), "rows of 4 MiB and more are not supported");
   if (num_seqs == 0) return VTKV_OK;
@@ -725,6 +737,11 @@ int vtkv_evict_rows(const int64_t *k_ptrs, const int64_t *v_ptrs, float *weights
   VTKV_REQUIRE(keep_rows > 0 && recent_rows >= 0 && recent_rows <= keep_rows,
                "keep_rows %d must be positive and recent_rows %d between 0 and keep_rows", keep_rows, recent_rows);
   VTKV_REQUIRE(max_seq_len > 0, "max_seq_len must be > 0");
+  VTKV_REQUIRE(weights_apart(slot_stride, head_stride, num_slots, num_kv_heads, max_seq_len),
+               "weights of different slots and kv heads overlap");
+  const intptr_t lens_apart = (intptr_t)new_seq_lens - (intptr_t)seq_lens, lens_bytes = (intptr_t)num_seqs * 4;
+  VTKV_REQUIRE(lens_apart == 0 || lens_apart >= lens_bytes || -lens_apart >= lens_bytes,
+               "new_seq_lens must be seq_lens itself or apart from it");
   const int64_t need = vtkv_evict_rows_workspace_bytes(num_seqs, num_kv_heads, max_seq_len, keep_rows, recent_rows);
   if (need > 0 && (!workspace || workspace_bytes < need))
     return vtkv::fail(VTKV_ENOMEM, "workspace of %lld bytes needed, got %lld", (long long)need, (long long)workspace_bytes);

@@ -446,7 +446,8 @@ int vtkv_decode_append_attention(void *out, const void *q, const void *key, cons
 /* Adds to weights[slot, kv head, row] the attention that one query token per sequence pays to the row, summed over the
  * kv head's query heads: sum_h softmax_row(scale * q[b,h,:] . K_b[row, kv head, :] [+ alibi]) for row < seq_lens[b].
  *   weights    device float [num_slots, num_kv_heads, >= max_seq_len], slot_stride and head_stride in elements, rows
- *              contiguous; indexed by slot, so that it stays with a sequence from step to step
+ *              contiguous; indexed by slot, so that it stays with a sequence from step to step; rows of different
+ *              (slot, kv head) must not overlap
  *   seq_lens   device int32[num_seqs], at most max_seq_len (larger ones are cut off); 0 leaves the slot as it is
  *   slot_ids   device int64[num_seqs]; the slots of a call are distinct, a slot outside [0, num_slots) is skipped
  *   kv_dtype   q_dtype, VTKV_FP8_E4M3 with k_scale, or VTKV_INT4
@@ -466,7 +467,7 @@ int vtkv_accumulate_attention_weights(float *weights, int64_t slot_stride, int64
  * largest weights[slot, kv head, row] (of equal ones the first; NaN counts as largest).  With heavy = keep_rows -
  * recent_rows: rows below heavy that stay keep their places; the other rows that stay fill, in order, the places of the
  * evicted ones below heavy; the recent rows move to [heavy, keep_rows) in order.  weights moves with the rows and is
- * zero in [keep_rows, n).  new_seq_lens[b] = min(seq_lens[b], keep_rows) (may be seq_lens itself).  Rows in [keep_rows, n)
+ * zero in [keep_rows, n).  new_seq_lens[b] = min(seq_lens[b], keep_rows) (seq_lens itself, or apart from it).  Rows in [keep_rows, n)
  * of the ranges are left as they were.
  *   seq_lens   device int32[num_seqs], at most max_seq_len; slots are distinct, a sequence whose slot lies outside
  *              [0, num_slots) is skipped: its new length is its old one

@@ -75,6 +75,30 @@ def _per_sequence(num_seqs: int, seq_lens: torch.Tensor, slot_mapping: torch.Ten
             raise _C.VtkvError(_C.EINVAL, "seq_lens and slot_mapping hold one entry per sequence, contiguous")
 
 
+def _int4_rows(key: torch.Tensor, value: torch.Tensor, slot_m: torch.Tensor, slot_mapping: torch.Tensor,
+               seq_lens: Optional[torch.Tensor], cache_seq_lens: Optional[torch.Tensor], max_seq_len: int,
+               num_kv_heads: int, head_size: int):
+    """Keys and values of a batch on their way to or from 4-bit rows: every entry that the kernels look up is there.
+    Returns both as [tokens, heads, head_size]."""
+    if slot_m.dtype != torch.int64 or slot_mapping.dtype != torch.int64:
+        raise _C.VtkvError(_C.EINVAL, "slot_m and slot_mapping must be int64")
+    if slot_mapping.dim() != 1 or slot_m.shape != slot_mapping.shape:
+        raise _C.VtkvError(_C.EINVAL, "slot_m and slot_mapping must hold one entry per sequence")
+    batch = slot_mapping.shape[0]
+    for t in (seq_lens, cache_seq_lens):
+        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous()):
+            raise _C.VtkvError(_C.EINVAL, "seq_lens and cache_seq_lens must be int32 and contiguous")
+        if max_seq_len > 1 and (t is None or t.numel() < batch):
+            raise _C.VtkvError(_C.EINVAL, "seq_lens and cache_seq_lens must hold one entry per sequence")
+    if key.dtype != value.dtype or not (slot_m.is_contiguous() and slot_mapping.is_contiguous()):
+        raise _C.VtkvError(_C.EINVAL, "key and value must have one dtype, slot_m and slot_mapping be contiguous")
+    key = key.view(-1, num_kv_heads, head_size)
+    value = value.view(-1, num_kv_heads, head_size)
+    if key.shape[0] != value.shape[0] or (max_seq_len == 1 and key.shape[0] < batch):
+        raise _C.VtkvError(_C.EINVAL, "key and value must hold the same tokens, one per sequence where max_seq_len is 1")
+    return key, value
+
+
 def _on_current_device(*tensors) -> None:
     here = None
     for t in tensors:
@@ -429,19 +453,16 @@ def reshape_and_cache(
         _require_cuda(seq_lens, cache_seq_lens)
         _pointer_tables(key_cache, value_cache)
         _on_current_device(key, value, key_cache, value_cache, slot_m, slot_mapping, seq_lens, cache_seq_lens)
-        if any(t is not None and not t.is_contiguous() for t in (seq_lens, cache_seq_lens)):
-            raise _C.VtkvError(_C.EINVAL, "seq_lens and cache_seq_lens must be contiguous")
-        if key.dtype != value.dtype or not (slot_m.is_contiguous() and slot_mapping.is_contiguous()):
-            raise _C.VtkvError(_C.EINVAL, "key and value must have one dtype, slot_m and slot_mapping be contiguous")
-        if slot_m.shape != slot_mapping.shape:
-            raise _C.VtkvError(_C.EINVAL, "slot_m and slot_mapping must hold one entry per sequence")
-    if slot_m.dtype != torch.int64 or slot_mapping.dtype != torch.int64:
-        raise _C.VtkvError(_C.EINVAL, "slot_m and slot_mapping must be int64")
-    for t in (seq_lens, cache_seq_lens):
-        if t is not None and t.dtype != torch.int32:
-            raise _C.VtkvError(_C.EINVAL, "seq_lens and cache_seq_lens must be int32")
-    key = key.view(-1, num_kv_heads, head_size)
-    value = value.view(-1, num_kv_heads, head_size)
+        key, value = _int4_rows(key, value, slot_m, slot_mapping, seq_lens, cache_seq_lens, max_seq_len, num_kv_heads,
+                                head_size)
+    else:
+        if slot_m.dtype != torch.int64 or slot_mapping.dtype != torch.int64:
+            raise _C.VtkvError(_C.EINVAL, "slot_m and slot_mapping must be int64")
+        for t in (seq_lens, cache_seq_lens):
+            if t is not None and t.dtype != torch.int32:
+                raise _C.VtkvError(_C.EINVAL, "seq_lens and cache_seq_lens must be int32")
+        key = key.view(-1, num_kv_heads, head_size)
+        value = value.view(-1, num_kv_heads, head_size)
     if key.stride(2) != 1 or key.stride(1) != head_size or value.stride(2) != 1 or value.stride(1) != head_size:
         raise _C.VtkvError(_C.EINVAL, "key/value rows must be contiguous in (head, dim)")
     sd = _dt(key)
@@ -474,15 +495,7 @@ def read_cached_rows(
     _require_cuda(key, value, slot_m, slot_mapping, seq_lens, cache_seq_lens)
     _pointer_tables(key_cache, value_cache)
     _on_current_device(key, value, key_cache, value_cache, slot_m, slot_mapping, seq_lens, cache_seq_lens)
-    if slot_m.dtype != torch.int64 or slot_mapping.dtype != torch.int64 or slot_m.shape != slot_mapping.shape:
-        raise _C.VtkvError(_C.EINVAL, "slot_m and slot_mapping must be int64, one entry per sequence")
-    for t in (seq_lens, cache_seq_lens):
-        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous()):
-            raise _C.VtkvError(_C.EINVAL, "seq_lens and cache_seq_lens must be int32 and contiguous")
-    if key.dtype != value.dtype or not (slot_m.is_contiguous() and slot_mapping.is_contiguous()):
-        raise _C.VtkvError(_C.EINVAL, "key and value must have one dtype, slot_m and slot_mapping be contiguous")
-    key = key.view(-1, num_kv_heads, head_size)
-    value = value.view(-1, num_kv_heads, head_size)
+    key, value = _int4_rows(key, value, slot_m, slot_mapping, seq_lens, cache_seq_lens, max_seq_len, num_kv_heads, head_size)
     if key.stride(2) != 1 or key.stride(1) != head_size or value.stride(2) != 1 or value.stride(1) != head_size:
         raise _C.VtkvError(_C.EINVAL, "key/value rows must be contiguous in (head, dim)")
     _C.check(_C.lib().vtkv_read_cached_rows(

@@ -3,8 +3,9 @@ are turned away before a kernel is launched."""
 import ctypes as C
 
 import pytest
+import torch
 
-from glake_amd import _C
+from glake_amd import _C, _custom_ops as ops
 from test_small_cache_refusals import P, evict, refused, weigh
 
 N = C.c_void_p(0)
@@ -36,3 +37,24 @@ def test_lengths_that_overlap_in_part_are_refused():
     # (apart or the same: refused only for the workspace that is missing here)
     for n in (0, 16, -16):
         assert evict(sl=P, nl=at(n), b=4, ws=N) == _C.ENOMEM
+
+
+def rows(tokens=4, values=4, batch=4, lens=4, starts=4, most=3, offsets=None):
+    key, value = torch.zeros(tokens, 2, 64), torch.zeros(values, 2, 64)
+    i64, i32 = torch.zeros(batch, dtype=torch.int64), torch.zeros(16, dtype=torch.int32)
+    return ops._int4_rows(key, value, i64 if offsets is None else torch.zeros(offsets, dtype=torch.int64), i64,
+                          None if lens is None else i32[:lens], None if starts is None else i32[:starts], most, 2, 64)
+
+
+@pytest.mark.parametrize("kw", [dict(lens=3), dict(starts=3), dict(lens=None), dict(starts=None), dict(values=3), dict(tokens=3),
+                                dict(offsets=3), dict(most=1, tokens=3, values=3)])
+def test_rows_without_an_entry_for_every_sequence_are_refused(kw):
+    with pytest.raises(_C.VtkvError):
+        rows(**kw)
+
+
+@pytest.mark.parametrize("kw", [{}, dict(lens=9, starts=5), dict(tokens=100, values=100), dict(most=1, lens=None, starts=None),
+                                dict(most=1, tokens=6, values=6, lens=1), dict(batch=0, lens=0, starts=0), dict(tokens=2, values=2)])
+def test_rows_with_an_entry_for_every_sequence(kw):
+    key, value = rows(**kw)
+    assert key.shape[1:] == value.shape[1:] == (2, 64)

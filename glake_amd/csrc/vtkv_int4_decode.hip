@@ -966,7 +966,7 @@ int int4_decode(void *out, const void *q, const int64_t *k_ptrs, const int64_t *
   p.out_f32 = out_dtype == VTKV_F32;
   p.scale_log2 = scale * kLog2e;
   const int j = p.group <= 8 ? 2 : 1;
-  for (int at = 0; at < num_seqs; at += kMaxBatch) {
+  for (int at = 0; at < num_seqs; at += p.num_seqs) {
     p.num_seqs = std::min(kMaxBatch, num_seqs - at);
     p.q = (const uint16_t *)q + at * q_stride;
     p.slot_ids = slot_ids + at;
@@ -975,6 +975,10 @@ int int4_decode(void *out, const void *q, const int64_t *k_ptrs, const int64_t *
     size_t lds;
     const int planned = plan(p, head_size, num_kv_heads, lds);
     if (planned < 0) return planned;
+    // (a launch numbers its units with 32 bits)
+    const int64_t most = 0x7fffffff / ((((int64_t)max_seq_len - 1) / kUnitRows + 1 + p.part_units) * p.chunks);
+    VTKV_REQUIRE(most > 0, "max_seq_len %d is too large for %d kv heads", max_seq_len, num_kv_heads);
+    p.num_seqs = (int)std::min<int64_t>(p.num_seqs, most);
     const int64_t table = ((int64_t)p.num_seqs * p.chunks * 8 + 63) / 64 * 64;
     const int64_t per_span = 2ll * p.chunk_heads * p.group * (head_size + 2) * 4;
     const int64_t room = workspace ? (workspace_bytes - table) / per_span : 0;

@@ -253,3 +253,20 @@ def test_empty_sequences_may_have_any_slot(env):
     before = r.k.clone()
     ops.reshape_and_cache(key, key, r.kp, r.vp, i64([-1] * b), i64([-1] * b), None, None, 1, hkv, d, "int4")
     assert torch.equal(r.k, before)
+
+
+def test_decode_of_a_batch_that_takes_several_launches(env):
+    """A loose bound on the lengths and many chunks of kv heads: the units of all sequences together pass 32 bits, so the
+    batch runs in parts."""
+    torch, ops = env
+    rng = np.random.default_rng(52)
+    hkv, d, b = 37, 64, 25
+    lens = [int(n) for n in rng.integers(0, 60, b)]
+    r, k, v = filled(rng, lens, hkv, d)
+    q, qh = S.as_type(rng.standard_normal((b, hkv, d)), torch.bfloat16)
+    out = torch.full(q.shape, 55.0, device="cuda")
+    ops.paged_attention_v1(out, q, r.kp, r.vp, hkv, d ** -0.5, i32(lens), 1, 100_000_000, None, "int4", 1.0, i64(list(range(b))))
+    for i, n in enumerate(lens):
+        want = S.attention(qh[i:i + 1], k[i], v[i], d ** -0.5)[0] if n else np.zeros((hkv, d))
+        top = np.abs(v[i]).max() if n else 0.0
+        assert (np.abs(out[i].double().cpu().numpy() - want) <= 2.0 ** -12 * top).all()

@@ -58,3 +58,10 @@ def test_rows_without_an_entry_for_every_sequence_are_refused(kw):
 def test_rows_with_an_entry_for_every_sequence(kw):
     key, value = rows(**kw)
     assert key.shape[1:] == value.shape[1:] == (2, 64)
+
+
+def test_more_units_than_a_launch_can_number():
+    from test_small_cache_refusals import decode
+
+    refused(decode(h=17, hk=17, qs=17 * 128, m=0x7fffffff), "max_seq_len")
+    assert decode(h=17, hk=17, qs=17 * 128, m=1 << 30) == _C.ENOMEM  # (only the workspace is missing)

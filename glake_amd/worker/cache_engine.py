@@ -64,8 +64,8 @@ class CacheEngine:
                  max_num_batched_tokens: int, cache_seqs: int = 0, cache_tokens: int = 0,
                  swap_space_bytes: int = 0, device: int = 0, value_skew: int = 256,
                  kv_cache_dtype: Optional[str] = None) -> None:
-        """``dtype``: the rows' element type (torch.uint8: an fp8 cache).  ``kv_cache_dtype="int4"``: 4-bit rows,
-        whatever ``dtype`` the model has."""
+        """``dtype``: the rows' element type (torch.uint8: an fp8 cache).  ``kv_cache_dtype="int4"``: 4-bit rows
+        of a bfloat16 or float16 model (``dtype`` then says nothing about the rows)."""
         self.num_layers = num_layers
         self.num_kv_heads = num_kv_heads
         self.head_size = head_size

@@ -270,3 +270,123 @@ def test_decode_of_a_batch_that_takes_several_launches(env):
         want = S.attention(qh[i:i + 1], k[i], v[i], d ** -0.5)[0] if n else np.zeros((hkv, d))
         top = np.abs(v[i]).max() if n else 0.0
         assert (np.abs(out[i].double().cpu().numpy() - want) <= 2.0 ** -12 * top).all()
+
+
+# ------------------------------------------------------------------------------------------------ the attention weights
+@pytest.mark.parametrize("kind", ["auto", "fp8", "int4"])
+@pytest.mark.parametrize("fit", [1, 2, 4])
+def test_weights_through_a_workspace_of_a_few_sequences(env, kind, fit):
+    """A workspace that holds some of the batch's sequences: the parts run one after the other through it, bit for bit as all
+    at once."""
+    import ctypes as C
+
+    from glake_amd import _C
+
+    torch, _ = env
+    rng = np.random.default_rng(60)
+    lens, hq, hkv, d = [300, 1, 0, 129, 700, 64, 65], 8, 2, 128
+    b, most = len(lens), max(lens)
+    if kind == "int4":
+        r, _, _ = filled(rng, [max(n, 1) for n in lens], hkv, d)
+    else:
+        r = S.Ranges(b, most, hkv * d * (1 if kind == "fp8" else 2))
+        x = torch.from_numpy(rng.standard_normal((b, most, hkv * d)).astype(np.float32))
+        r.k[:] = x.to(torch.float8_e4m3fn if kind == "fp8" else torch.bfloat16).view(torch.uint8).view(r.k.shape).cuda()
+    q = torch.from_numpy(rng.standard_normal((b, hq, d)).astype(np.float32)).bfloat16().cuda()
+    lib = _C.lib()
+    slots, lens_t = i64(list(reversed(range(b)))), i32(list(reversed(lens)))
+    one = lib.vtkv_accumulate_attention_weights_workspace_bytes(1, hq, most)
+    got = []
+    for nbytes in (one * b, one * fit + 16):
+        w = torch.zeros(b, hkv, most, device="cuda")
+        ws = torch.full((nbytes,), 0xFF, dtype=torch.uint8, device="cuda")
+        p = lambda t: C.c_void_p(t.data_ptr())  # noqa: E731
+        _C.check(lib.vtkv_accumulate_attention_weights(
+            p(w), w.stride(0), w.stride(1), b, p(q), p(r.kp), p(slots), p(lens_t), b, hq, hkv, d, hq * d, d ** -0.5, most, None,
+            _C.BF16, {"auto": _C.BF16, "fp8": _C.FP8_E4M3, "int4": _C.INT4}[kind], 1.0, p(ws), nbytes,
+            C.c_void_p(torch.cuda.current_stream().cuda_stream)))
+        got.append(w)
+    assert torch.equal(*got)
+    sums = got[0].double().sum(-1).cpu().numpy()  # (each query head pays 1 in all: 700 rows within 2^-12 of themselves)
+    assert (np.abs(sums - np.array([hq // hkv if n else 0 for n in lens])[:, None]) <= hq // hkv * 2.0 ** -11).all()
+
+
+# ------------------------------------------------------------------------------------------------ a bounded cache, served
+@pytest.mark.parametrize("kind", ["auto", "int4"])
+@pytest.mark.parametrize("path", ["plan", "backend"])
+def test_a_bounded_cache_on_the_engine(env, gpu_pool, kind, path):
+    """Prompts through the backend, then decode steps through a DecodeStepPlan or the backend over a CacheEngine's ranges,
+    weights after each step, evictions when a sequence is four rows over its budget.  The lengths that the calls take are
+    numbers of rows, not of tokens, from the first eviction on."""
+    torch, ops = env
+    from glake_amd.attention.backends.vtensor import VTensorImpl
+    from glake_amd.worker.cache_engine import CacheEngine
+    from glake_amd.worker.step import DecodeStepPlan, prepare_step
+
+    rng = np.random.default_rng(61)
+    hq, hkv, d, keep, recent, slack, room = 8, 2, 128, 40, 12, 4, 64
+    slots, lens = [2, 0], [39, 30]
+    eng = CacheEngine(1, hkv, d, torch.bfloat16, 3, 4096, kv_cache_dtype=kind)
+    impl = VTensorImpl(hq, d, d ** -0.5, hkv, kv_cache_dtype=kind)
+    segments = [eng.vmm_kvcache_segment[s] for s in slots]
+    tables = eng.k_cache_ptr[0], eng.v_cache_ptr[0]
+    weights = torch.zeros(3, hkv, room, device="cuda")
+    held = [[[np.zeros((0, d))] * hkv for _ in range(2)] for _ in slots]  # [sequence][K, V][head] -> rows
+
+    def batch(n_new):
+        out = []
+        for _ in range(2):
+            t, h = S.as_type(S.model_values(rng, (sum(n_new), hkv, d)), torch.bfloat16)
+            out.append((t, S.values(*S.quantise(h)) if kind == "int4" else h))
+        at = 0
+        for i, n in enumerate(n_new):
+            for side in range(2):
+                held[i][side] = [np.concatenate([x, out[side][1][at:at + n, h]]) for h, x in enumerate(held[i][side])]
+            at += n
+        q, qh = S.as_type(rng.standard_normal((sum(n_new), hq, d)), torch.bfloat16)
+        return q, qh, out[0][0], out[1][0]
+
+    def through_backend(q, k, v, rows, prompt):
+        meta = S.step_metadata(eng, slots, rows, prompt)
+        prepare_step(meta, eng.gpu_cache)
+        return impl.forward(q.view(-1, hq * d), k.view(-1, hkv * d), v.view(-1, hkv * d), *eng.gpu_cache[0], meta).view(-1, hq, d)
+
+    def compare(out, qh, n_new, bound):
+        at = 0
+        for i, n in enumerate(n_new):
+            kk, vv = (np.stack(held[i][s], 1) for s in range(2))
+            want = S.attention(qh[at:at + n], kk, vv, d ** -0.5, np.arange(len(kk) - n, len(kk)) + 1)
+            err = np.abs(out[at:at + n].double().cpu().numpy() - want)
+            assert (err <= bound * np.abs(vv).max() + 2.0 ** -8 * np.abs(want)).all()
+            at += n
+
+    q, qh, k, v = batch(lens)
+    compare(through_backend(q, k, v, lens, True), qh, lens, 2.0 ** -10 + 2.0 ** -11)
+    plan = DecodeStepPlan(segments, slots, *tables, hq, hkv, d, d ** -0.5, kv_cache_dtype=kind)
+    evictions = 0
+    for _ in range(30):
+        q, qh, k, v = batch([1, 1])
+        rows = [len(held[i][0][0]) for i in range(2)]
+        if path == "plan":
+            out = torch.empty_like(q)
+            assert plan.run(q, k, v, out) == max(rows) and plan.seq_lens.tolist() == rows
+        else:
+            out = through_backend(q, k, v, rows, False)
+        compare(out, qh, [1, 1], 2.0 ** -12)
+        lens_t = i32(rows)
+        ops.accumulate_attention_weights(weights, q, tables[0], hkv, d ** -0.5, lens_t, max(rows), i64(slots), None, kind)
+        if max(rows) < keep + slack:
+            continue
+        evictions += 1
+        before = weights.double().cpu().numpy()
+        ops.evict_rows(*tables, weights, lens_t, lens_t, keep, recent, max(rows), i64(slots), hkv, d, kind)
+        for i, n in enumerate(lens_t.tolist()):
+            assert n == min(rows[i], keep)
+            segments[i].set_used_size(n * eng.token_size)
+            for h in range(hkv):
+                src = S.evicted_sources(before[slots[i], h, :rows[i]], rows[i], keep, recent)
+                for side in range(2):
+                    held[i][side][h] = held[i][side][h][src]
+    assert evictions >= 4 and all(s.used_size == len(held[i][0][0]) * eng.token_size for i, s in enumerate(segments))
+    torch.cuda.synchronize()
+    eng.close()

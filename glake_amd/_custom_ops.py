@@ -570,9 +570,10 @@ def evict_rows(
     rows move to ``[heavy, keep_rows)``.  ``weights`` moves with the rows and is zero behind them; ``new_seq_lens``
     (which may be ``seq_lens``) receives the lengths.  The slots of a call are distinct; a sequence whose slot the weights or
     a pointer table do not have is skipped and keeps its length.  The caller takes the rows off its own bookkeeping
-    (``KVcacheSegment.set_used_size``); later calls take numbers of rows for its lengths, not of tokens.  The rows of a head are not in the order of their tokens afterwards, which
-    attention without ALiBi does not notice; ranges that share chunks with another sequence must not be evicted from.
-    ``model_dtype`` is the type of the rows of an "auto" cache.  No counterpart in the reference."""
+    (``KVcacheSegment.set_used_size``); later calls take numbers of rows for its lengths, not of tokens.  The rows of a
+    head are not in the order of their tokens afterwards, which attention without ALiBi does not notice; ranges that
+    share chunks with another sequence must not be evicted from.  ``model_dtype`` is the type of the rows of an "auto"
+    cache.  No counterpart in the reference."""
     _require_cuda(weights, new_seq_lens)
     num_seqs = slot_mapping.shape[0]
     _per_sequence(num_seqs, seq_lens, slot_mapping)

@@ -718,7 +718,9 @@ __global__ void __launch_bounds__(waves_of(D) * 64) int4_decode_kernel(DecodePar
 // Attention of one query head over the values themselves, in fp32 on the vector unit by a workgroup of 256 threads: for
 // results that the kernel above could not hold (and for those that are not finite whichever way they are computed).  A thread
 // takes whole rows for their logits, then, 256 rows at a time, a dim for the sum of the values, whose weights are normalised
-// first: it stays as small as the values are.
+// first: it stays as small as the values are.  Where a logit or a V row is not a number the result is none either, and known
+// after the logits.  (One sequence of 131072 rows, 32 query heads over 8 kv heads of
+// 128: 12 ms, 1.3 ms where it ends after the logits; ordinary values take 0.1 ms.)
 template <int D, bool F16>
 __device__ void plain_attention(const DecodeParams &p, int b, int head, int len) {
   __shared__ float s_q[D], s_p[256], s_top[256];
@@ -735,7 +737,7 @@ __device__ void plain_attention(const DecodeParams &p, int b, int head, int len)
     const unsigned pair = *reinterpret_cast<const unsigned *>(row + pair_at);
     const float s = __builtin_bit_cast(float, pair << 16), z = __builtin_bit_cast(float, pair & 0xffff0000u);
     float x = 0.f;
-#pragma unroll 1
+#pragma unroll 4
     for (int w = 0; w < D / 8; ++w)
 #pragma unroll
       for (int i = 0; i < 8; ++i)
@@ -744,12 +746,16 @@ __device__ void plain_attention(const DecodeParams &p, int b, int head, int len)
   };
   // ---- maximum and sum
   float m = -INFINITY, l = 0.f;
+  bool none = false;
 #pragma unroll 1
   for (int r = tid; r < len; r += 256) {
+    const unsigned pair = *reinterpret_cast<const unsigned *>(v_rows + (int64_t)r * p.row_bytes + pair_at);
     const float x = logit(r), top = fmaxf(m, x);
-    l = l * (m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top)) + __builtin_amdgcn_exp2f(x - top);
+    none |= (pair & 0x7f80u) == 0x7f80u || (pair & 0x7f800000u) == 0x7f800000u || x != x || x == INFINITY;
+    l = l * (m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top)) + (x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x - top));
     m = top;
   }
+  none = __syncthreads_or(none);
   s_top[tid] = m;
   __syncthreads();
   float all = -INFINITY;
@@ -760,15 +766,15 @@ __device__ void plain_attention(const DecodeParams &p, int b, int head, int len)
   for (int i = 0; i < 256; ++i) sum += s_p[i];
   const float inv = 1.f / sum;
   // ---- the values
-  float o = 0.f;
+  float o = none ? __builtin_nanf("") : 0.f;
 #pragma unroll 1
-  for (int r0 = 0; r0 < len; r0 += 256) {
+  for (int r0 = 0; r0 < len && !none; r0 += 256) {
     __syncthreads();
     if (r0 + tid < len) s_p[tid] = __builtin_amdgcn_exp2f(logit(r0 + tid) - all) * inv;
     __syncthreads();
     if (tid < D) {
       const char *row = v_rows + (int64_t)r0 * p.row_bytes;
-#pragma unroll 1
+#pragma unroll 8
       for (int i = 0; i < min(256, len - r0); ++i, row += p.row_bytes) {
         const unsigned pair = *reinterpret_cast<const unsigned *>(row + pair_at), code = (unsigned char)row[codes_at + tid / 2] >> (4 * (tid & 1)) & 15u;
         o = __builtin_fmaf(s_p[i], __builtin_fmaf((float)code, __builtin_bit_cast(float, pair << 16), __builtin_bit_cast(float, pair & 0xffff0000u)), o);

@@ -64,7 +64,7 @@ __device__ __forceinline__ float other_part(float x) {
 // KV: 0: 16-bit rows of the model's type, 1: e4m3fn codes, 2: 4-bit rows.  A wave takes up to kTiles tiles of 64 rows
 // of one kv head one after the other; while a tile is multiplied, the next one is on its way.  The workgroup's waves take
 // kv heads next to each other of the same rows, since a head's part of a row is short (64 sequences of 512 to 4096 rows,
-// 32 query heads over 8 kv heads of 128 bf16 elements: 68 us that way, 5.0 TB/s; four waves along the rows of one head: 82 us).
+// 32 query heads over 8 kv heads of 128 bf16 elements: 68 us that way, K at 4.5 TB/s; four waves along the rows of one head: 82 us).
 //  * 16-bit and fp8 rows go into the wave's own LDS as whole head rows (a load instruction covers whole cache lines; lane m
 //    of an MFMA operand holds one row, so loads into registers would take 64 bytes of sixteen rows each: 88 us against 82),
 //    from there into registers, which frees the LDS for the next tile.  Rows of a power of two of 16-byte pieces have their

@@ -35,9 +35,9 @@
 // the end of a part took 4.5 us; two stages 35 us, four 32 us).  A span that ends inside a sequence leaves a partial
 // result in the workspace and a second kernel merges them.
 //
-// What it takes (kernel and merge): 64 sequences of 512 to 4096 rows of 8 kv heads of 128, 4 query heads each (161 MB): 43 + 5
-// us; four of 32768 to 131072 rows (371 MB): 77 + 5 us; 32 kv heads of 80 as above (60 MB): 30 + 4 us; one of 777 rows: 16 + 4
-// us.  A stage takes 2.85 us with all workgroups at it (6.3 TB/s), the way to the first stage's rows 8.5 us, the end of a
+// What it takes (kernel and merge): 64 sequences of 512 to 4096 rows of 8 kv heads of 128, 4 query heads each (161 MB): 44 + 6
+// us; four of 32768 to 131072 rows (371 MB): 80 + 5 us; 32 kv heads of 80 as above (60 MB): 31 + 4 us; one of 777 rows: 16 + 4
+// us.  A stage takes 3.0 us with all workgroups at it (6.0 TB/s), the way to the first stage's rows 8.8 us, the end of a
 // part 2.5 to 4 us.
 #include "vtkv_attn_common.h"
 #include "vtkv_common.h"

@@ -4,8 +4,8 @@
 // maximum over the team, one division for the scale, eight codes packed into one 4-byte store.  A workgroup takes four
 // tokens, whose K and V heads its teams share out, four loads of a team in flight.
 //   The bytes of the 16-bit rows bound it (about 4/5 of what moves), writing also the 30 instructions per value, at
-// decode-step sizes the launch.  16 000 tokens of 8 kv heads of 128 (67 MB of 16-bit rows, 18 MB of 4-bit ones): written in
-// 27 us, 3.1 TB/s, read back in 21 us, 4.0 TB/s; with one token per workgroup 42 and 32 us, with two 29 and 24, with eight
+// decode-step sizes the launch.  15 800 tokens of 8 kv heads of 128 (65 MB of 16-bit rows, 17 MB of 4-bit ones): written in
+// 27 us, 3.0 TB/s, read back in 21 us, 3.9 TB/s; with one token per workgroup 42 and 32 us, with two 29 and 24, with eight
 // as with four.
 #include "vtkv_common.h"
 #include "vtkv_fp8.h"

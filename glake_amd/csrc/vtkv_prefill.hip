@@ -27,13 +27,13 @@
 //    to bf16 and V to fp16 (both exactly), so everything after the stage is the bf16 kernel; the K scale
 //    folds into the logit scale and the V scale into the final normalisation.
 //  * 4-bit cache (vtkv_int4.h): K goes into the stage as bare codes, two masks per pair of them (fp16 denormals c * 2^-24
-//    and c * 2^-20; the queries are brought to fp16 by a power of two and carry the rest, each column by its own where they are far
-//    apart), so S runs on the fp16 MFMA for either model type; a row's scale and zero, kept beside the stage, turn its dot products into
-//    logits: x = scale (q . c) + zero sum(q).  V is converted on its way in, c * scale + zero in one rounding to fp16
+//    and c * 2^-20; the queries are brought to fp16 by a power of two and carry the rest, each column by its own where they
+//    are far apart), so S runs on the fp16 MFMA for either model type; a row's scale and zero, kept beside the stage, turn its
+//    dot products into logits: x = scale (q . c) + zero sum(q).  V is converted on its way in, c * scale + zero in one rounding to fp16
 //    (2^-12 of the value), the dims in the order in which pairs of codes come out of a word; scales from 128 and zeros
 //    beyond the fp16 range take the second pass like large bf16 values, there rounded to bf16.  The conversion is what it
-//    costs over the others: eight prompts of 2048 tokens, 32 heads over 8 of 128: 391 us (0.70 PFLOP/s) against 337 us from
-//    a bf16 cache; four chunks of 300 to 700 tokens behind 2000 to 7000 rows, 64 heads: 485 us (0.79) against 405 us.
+//    costs over the others: eight prompts of 2048 tokens, 32 heads over 8 of 128: 384 us (0.72 PFLOP/s) against 337 us from
+//    a bf16 cache; four chunks of 301 to 700 tokens behind 2000 to 7200 rows, 64 heads: 503 us (0.72) against 405 us.
 //
 // Otherwise numerics as in the decode kernel (vtkv_attention.hip); the reference computes this with xformers /
 // an external flash-attention kernel (vllm/attention/backends/xformers.py:331-386).

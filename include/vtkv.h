@@ -409,7 +409,7 @@ int vtkv_prefill_unit_tokens(int num_heads, int num_kv_heads, int kv_dtype);
  * VTKV_BF16 or VTKV_F16, kv_dtype = q_dtype or VTKV_FP8_E4M3 with k_scale / v_scale, out_dtype = q_dtype or
  * VTKV_F32; the longest-units-first order inside each sequence, sequence by sequence, lets every row be fetched
  * from HBM once.  Values of V are carried in fp16 (below 2^-14 they lose bits, below 2^-25 they vanish); a unit that meets
- * larger ones than fp16 holds is computed again with them in bf16.  q_dtype VTKV_F32 with kv_dtype = out_dtype = VTKV_F32 (float32 models): every token attends
+ * larger ones than fp16 holds (4-bit rows: scales from 128) is computed again with them in bf16.  q_dtype VTKV_F32 with kv_dtype = out_dtype = VTKV_F32 (float32 models): every token attends
  * through the float32 decode kernel by itself, without reuse of rows between tokens. */
 int vtkv_prefill_attention(void *out, const void *q, const int64_t *k_ptrs, const int64_t *v_ptrs,
                            const int64_t *slot_ids, const int32_t *units, int num_units, int num_heads,
@@ -496,7 +496,7 @@ int vtkv_set_head_major(int on);
 
 /* Benchmark aid without a counterpart in the reference (its kernel benchmark times from the host,
  * benchmarks/kernels/benchmark_paged_attention.py:147-157): while switched on, each vtkv_decode_attention
- * call (up to 1024 of them) launches its kernels with a start and a stop HIP event each on the caller's
+ * call over a 16-bit or fp8 cache (up to 1024 of them) launches its kernels with a start and a stop HIP event each on the caller's
  * stream (the begin and the end of that kernel's own dispatch, as a kernel trace reports them) without
  * waiting for them.  vtkv_attention_kernel_times waits for the recorded calls and writes, for the first
  * min(capacity, calls) of them in call order, the duration of the streaming kernel and of the merge

@@ -385,6 +385,8 @@ __global__ void __launch_bounds__(kThreads) prefill_attn_kernel(PrefillParams p)
           // times NaN would do that to those that do not
           const bool bad = (v_pair[j] & 0x7f80u) == 0x7f80u || (v_pair[j] & 0x7f800000u) == 0x7f800000u;
           if (bad) s = z = 0.f;
+          s *= 0x1p-32f;  // (so that weights of up to 2^8 each times values near the end of the fp32 range add up within it)
+          z *= 0x1p-32f;
           if (ld_piece[j] == 0) s_pairs[decltype(bufc)::value][2][ld_row[j]] = bad ? 1.f : 0.f;
           *reinterpret_cast<u32x4 *>(base + st_v[j]) = codes_to_bf16(vst[j][0], s, z);
           *reinterpret_cast<u32x4 *>(base + (st_v[j] ^ 16)) = codes_to_bf16(vst[j][1], s, z);
@@ -622,6 +624,7 @@ __global__ void __launch_bounds__(kThreads) prefill_attn_kernel(PrefillParams p)
     }
   };
   run(std::false_type{});
+  float v_back = p.v_scale;
 #ifdef VTKV_PREFILL_TRACE
   const unsigned long long trace_t2 = wall_clock64();
 #endif
@@ -654,6 +657,7 @@ __global__ void __launch_bounds__(kThreads) prefill_attn_kernel(PrefillParams p)
       reset();
       rewind();
       run(std::true_type{});
+      if constexpr (I4) v_back = 0x1p32f;
     }
   }
 
@@ -662,7 +666,7 @@ __global__ void __launch_bounds__(kThreads) prefill_attn_kernel(PrefillParams p)
 #pragma unroll
   for (int nb = 0; nb < kNB; ++nb) {
     const float l = acc_l[nb][0];  // (already the sum over all rows: see acc_l)
-    float inv = p.v_scale / l;
+    float inv = v_back / l;
     if (I4 && wave_max_over_row_groups(sees_bad[nb]) > 0.f) inv = __builtin_nanf("");
     if (col_tok[nb] < 0) continue;
     const int64_t o0 = ((int64_t)(u_row0 + col_tok[nb]) * p.num_heads + head0 + col_head[nb]) * kD +

@@ -197,6 +197,24 @@ def test_decode_of_small_values(env, factor):
         assert (np.abs(got[i].double().cpu().numpy() - want) <= 2.0 ** -12 * np.abs(v[i]).max()).all()
 
 
+@pytest.mark.parametrize("factor", [1e6, 1e30, 1e37])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_prompt_of_large_finite_values(env, dtype, factor):
+    """Values that a unit's second pass holds as bfloat16: half a step, 2^-8 of the largest value at most."""
+    torch, ops = env
+    rng = np.random.default_rng(45)
+    lens, hq, hkv, d = [130, 60], 8, 2, 128
+    r, k, v = filled(rng, lens, hkv, d, v_factor=factor)
+    q, qh = S.as_type(rng.standard_normal((sum(lens), hq, d)) * 3, torch.float16 if dtype == "fp16" else torch.bfloat16)
+    out = torch.empty(q.shape, device="cuda")
+    ops.prefill_attention(out, q, r.kp, r.vp, hkv, d ** -0.5, lens, lens, i64([0, 1]), None, "int4")
+    at = 0
+    for i, n in enumerate(lens):
+        want = S.attention(qh[at:at + n], k[i], v[i], d ** -0.5, np.arange(n) + 1)
+        assert (np.abs(out[at:at + n].double().cpu().numpy() - want) <= 2.0 ** -8 * np.abs(v[i]).max()).all()
+        at += n
+
+
 # ------------------------------------------------------------------------------------------------ slots
 @pytest.mark.parametrize("alias", [False, True])
 @pytest.mark.parametrize("kind", ["auto", "int4"])

@@ -659,6 +659,7 @@ int vtkv_accumulate_attention_weights(float *weights, int64_t slot_stride, int64
   VTKV_REQUIRE(max_seq_len > 0 && num_slots > 0, "max_seq_len and num_slots must be > 0");
   VTKV_REQUIRE(weights_apart(slot_stride, head_stride, num_slots, num_kv_heads, max_seq_len),
                "weights of different slots and kv heads overlap");
+  VTKV_REQUIRE(max_seq_len <= 1 << 30, "max_seq_len %d is too large", max_seq_len);  // (rows are numbered with 32 bits)
   VTKV_REQUIRE(num_heads <= 65535, "too many query heads");
   VTKV_REQUIRE(vtkv_kv_row_bytes(num_kv_heads, head_size, kv_dtype) < (4 << 20), "rows of 4 MiB and more are not supported");
   if (num_seqs == 0) return VTKV_OK;

@@ -65,3 +65,9 @@ def test_more_units_than_a_launch_can_number():
 
     refused(decode(h=17, hk=17, qs=17 * 128, m=0x7fffffff), "max_seq_len")
     assert decode(h=17, hk=17, qs=17 * 128, m=1 << 30) == _C.ENOMEM  # (only the workspace is missing)
+
+
+def test_more_rows_than_the_weights_can_number():
+    one = dict(h=1, hk=1, ss=1 << 40, hs=1 << 40, ns=1)
+    refused(weigh(m=0x7fffffff, b=0, **one), "max_seq_len")
+    assert weigh(m=1 << 30, b=0, **one) == 0

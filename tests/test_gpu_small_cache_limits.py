@@ -75,7 +75,7 @@ def filled(rng, lens, hkv, d, k_factor=1.0, v_factor=1.0):
 
 
 @pytest.mark.parametrize("value", [2.0 ** 26, 1e30])
-@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (16, 1, 80), (8, 8, 64)])
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (16, 1, 80), (8, 8, 64), (6, 2, 256), (40, 2, 112)])
 def test_a_large_query_stays_with_its_head(env, value, hq, hkv, d):
     """One large finite number in one head of one token: decode, prompts and weights are, everywhere else, as they are
     without it, and that head attends to the one row that is largest there.  Tolerances as for ordinary values: 2^-12 of the
@@ -137,6 +137,27 @@ def test_decode_of_large_finite_values(env, lens, hq, hkv, d, factor):
         want = S.attention(qh[i:i + 1], k[i], v[i], d ** -0.5)[0]
         assert (np.abs(got[i].double().cpu().numpy() - want) <= 2.0 ** -12 * np.abs(v[i]).max()).all()
     assert torch.equal(got.bfloat16(), rounded)
+
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(40, 2, 128), (71, 1, 64), (8, 8, 96)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_decode_of_large_values_with_alibi_and_many_heads(env, dtype, hq, hkv, d):
+    torch, ops = env
+    rng = np.random.default_rng(46)
+    lens = [500, 1, 0, 257]
+    r, k, v = filled(rng, [max(n, 1) for n in lens], hkv, d, v_factor=1e32)
+    q, qh = S.as_type(rng.standard_normal((4, hq, d)), torch.float16 if dtype == "fp16" else torch.bfloat16)
+    slopes = np.abs(rng.standard_normal(hq)).astype(np.float32) * 0.05
+    out = torch.full(q.shape, 55.0, device="cuda")
+    ops.paged_attention_v1(out, q, r.kp, r.vp, hkv, d ** -0.5, i32(lens), 1, 900, torch.from_numpy(slopes).cuda(), "int4", 1.0,
+                           i64([0, 1, 2, 3]))
+    for i, n in enumerate(lens):
+        if n == 0:
+            assert (out[i] == 0).all()
+            continue
+        want = S.attention(qh[i:i + 1], k[i][:n], v[i][:n], d ** -0.5, [n], slopes)[0]
+        assert (np.abs(out[i].double().cpu().numpy() - want) <= 2.0 ** -12 * np.abs(v[i]).max()).all()
 
 
 @pytest.mark.parametrize("n", [100, 7000])
